@@ -76,6 +76,8 @@ typedef struct pk_hip_stats {
     uint64_t prefill_route_ns, prefill_gate_up_ns, prefill_down_ns;
     uint64_t q4_1_dispatches;
     uint64_t q5_0_dispatches, q5_1_dispatches, q2_k_dispatches, q3_k_dispatches;
+    uint64_t paged_plan_calls, paged_append_calls, paged_attention_calls;
+    uint64_t paged_plan_ns, paged_append_ns, paged_attention_ns;
 } pk_hip_stats;
 
 const char* pk_hip_version(void);
@@ -485,6 +487,143 @@ pk_hip_status pk_hip_attention_steps(pk_hip_ctx* ctx, const pk_hip_attention_con
                                      const float* q_norm, const float* k_norm, uint32_t steps,
                                      const float* q, const float* k, const float* v, float* out,
                                      char* error_buffer, size_t error_capacity);
+
+/* ---- Many requests over one paged KV cache ------------------------------------
+ * No counterpart in the reference, whose KvCache is one sequence's ring
+ * (src/kv_cache.cpp:131-294): here requests of any lengths share a pool of
+ * pages per layer.  A step is one plan (which pages and slots the new tokens
+ * take), then per layer an append (q/k head norms, rotation, K and V into the
+ * pages) and an attention of the new tokens over their requests' pages.
+ *
+ * Position p of request r lies in slot p % page_size of page
+ * block_table[r][p / page_size].  Pages are numbered below `pages`; a table
+ * entry that is not (PK_HIP_NO_PAGE) is a page that is not there: attention
+ * takes its positions as masked.  All buffers are device memory the caller owns;
+ * lengths live on the device, so a captured graph serves steps of any lengths
+ * within its bounds.  Optional pointers are NULL.  Scratch, streams and stream
+ * capture are as for pk_hip_moe_prefill_async; plan, append and attention of
+ * contexts of their own, or of one context on one stream, may be in flight at
+ * once. */
+#define PK_HIP_NO_PAGE 0xffffffffu
+#define PK_HIP_NO_SLOT 0xffffffffu
+
+/* One layer's cache: rows of head_dim values (64, 128 or 256) of type F16 (1) or
+ * BF16 (30); the row of (page, slot, head) starts page * page_stride + slot *
+ * slot_stride + head * head_stride elements from k and from v.  k and v are
+ * 16-byte aligned, strides multiples of 8; all three 0 mean rows packed as
+ * [page][slot][head].  page_size is a power of two up to 1024, pages * page_size
+ * below 2^31. */
+typedef struct pk_hip_paged_kv {
+    void* k;
+    void* v;
+    uint32_t type;
+    uint32_t pages, page_size, kv_heads, head_dim;
+    uint64_t page_stride, slot_stride, head_stride;
+} pk_hip_paged_kv;
+
+/* Bits of a plan's status[0]. */
+#define PK_HIP_PLAN_NO_PAGES 1u    /* more pages are needed than are free */
+#define PK_HIP_PLAN_TABLE_FULL 2u  /* a request outgrows its row of the block table */
+#define PK_HIP_PLAN_TOKENS 4u      /* more new tokens than max_tokens */
+#define PK_HIP_PLAN_STATE 8u       /* a stored length or the free count is out of range */
+
+/* From every request's cached and new lengths: the pages and slots of the new
+ * tokens.  First the pages of released requests go back on the free stack in
+ * request and table order (entries that are no page are left out), their
+ * lengths count as 0, and their rows may take new tokens at once; then each
+ * request's missing pages come off the stack's end, requests in order, and into
+ * its row.  Entries for no token (from query_start[requests] on) get position 0,
+ * PK_HIP_NO_SLOT and request 0xffffffff.  A plan that does not fit changes
+ * neither block_table nor free_pages: lens_out and free_count_out repeat the
+ * inputs, every token entry is empty, and status[0] says why (PK_HIP_PLAN_*). */
+typedef struct pk_hip_paged_plan {
+    uint32_t requests;           /* rows of block_table, 1 .. 8192 */
+    uint32_t pages, page_size;   /* as pk_hip_paged_kv */
+    uint32_t table_stride;       /* entries of a row; times page_size at most 2^30 */
+    uint32_t max_tokens;         /* entries per token output, 1 .. 2^24 */
+    const uint32_t* lens;        /* [requests] positions cached */
+    const uint32_t* new_lens;    /* [requests] new tokens, 0 for none */
+    const uint32_t* release;     /* [requests] non-zero: the request has ended; or NULL */
+    uint32_t* block_table;       /* [requests][table_stride], updated */
+    uint32_t* free_pages;        /* [pages], the free stack, updated */
+    const uint32_t* free_count;  /* [1] pages on it */
+    uint32_t* lens_out;          /* [requests] positions with the new ones; may be lens */
+    uint32_t* free_count_out;    /* [1]; may be free_count */
+    uint32_t* query_start;       /* [requests + 1] where each request's tokens start */
+    uint32_t* positions;         /* [max_tokens] */
+    uint32_t* slots;             /* [max_tokens] page * page_size + slot in it */
+    uint32_t* token_request;     /* [max_tokens] */
+    uint32_t* status;            /* [4]: PK_HIP_PLAN_* bits, tokens, pages taken, pages returned */
+} pk_hip_paged_plan;
+
+/* Enqueued on `stream` without synchronising (NULL = the context stream). */
+pk_hip_status pk_hip_paged_plan_async(pk_hip_ctx* ctx, const pk_hip_paged_plan* plan, void* stream,
+                                      char* error_buffer, size_t error_capacity);
+
+/* q, k and v rows of `tokens` tokens (type F32, F16 or BF16; [heads] or [kv_heads]
+ * of head_dim values, tokens a stride apart): every q and k head is normed as
+ * rms_norm (src/rms_norm.cpp:9-27) with q_norm / k_norm (F32 [head_dim]; NULL: not
+ * normed) and its first rotary_dim values turned as NeoX RoPE (pairs i and i +
+ * rotary_dim / 2, src/qwen3_moe_runner.cpp:141-172): pair i by the angle
+ * positions[axis_i][token] * rope_theta^(-2 i / rotary_dim), axis_i = pair_axis[i].
+ * q goes to q_out (type and heads as q; may be q), k and v, rounded to the nearest
+ * even, to the token's slot.  Tokens whose slot is not in the cache
+ * (PK_HIP_NO_SLOT) are left out altogether: their q_out row stays as it was.  The
+ * slots of one call differ. */
+typedef struct pk_hip_paged_append {
+    pk_hip_paged_kv cache;
+    uint32_t type;             /* of q, k, v and q_out */
+    uint32_t tokens;           /* 1 .. 2^24 */
+    uint32_t heads;            /* q heads; 0: no q */
+    uint32_t rotary_dim;       /* a multiple of 16 up to head_dim; 0: no rotation */
+    uint32_t axes;             /* rows of positions, 1 .. 4 */
+    float rms_eps, rope_theta;
+    const void *q, *k, *v;     /* 16-byte aligned */
+    void* q_out;
+    /* elements from one token's row to the next (0: rows packed); 16-byte multiples */
+    uint64_t q_stride, k_stride, v_stride, q_out_stride;
+    const float *q_norm, *k_norm;
+    const uint32_t* positions; /* [axes][position_stride] */
+    uint64_t position_stride;  /* 0: tokens */
+    const uint8_t* pair_axis;  /* host memory, [rotary_dim / 2]; NULL: axis 0 */
+    const uint32_t* slots;     /* [tokens] */
+} pk_hip_paged_append;
+
+pk_hip_status pk_hip_paged_append_async(pk_hip_ctx* ctx, const pk_hip_paged_append* append,
+                                        void* stream, char* error_buffer, size_t error_capacity);
+
+/* Causal attention of new tokens: rows query_start[r] .. query_start[r + 1] - 1 of q
+ * are the last positions of request r, whose lens[r] positions (these included) lie in
+ * its pages.  The row of position p sees position i if i <= p, i's page is there, and,
+ * with a window, i + window > p or i < sinks:
+ *   out = sum_i softmax_i(scale * q . k_i) v_i (KvCache::attend, src/kv_cache.cpp:
+ * 219-294), head h over kv head h / (heads / kv_heads), and 0 where nothing is seen.
+ * Decoding requests, chunks of prompts and requests without a row mix freely.  q and out
+ * are F32 (with either cache type) or of the cache's type; sums and the softmax are FP32
+ * (F32: q and the weights enter the products as two or three parts, else the weights are
+ * rounded to the cache's type).  Requests with more than max_new rows, and rows of no
+ * request, are left as they were.  What masked positions hold, NaN too, does not
+ * matter. */
+typedef struct pk_hip_paged_attention {
+    pk_hip_paged_kv cache;
+    uint32_t type;               /* of q and out */
+    uint32_t heads;              /* a multiple of cache.kv_heads */
+    uint32_t requests;           /* 1 .. 8192 */
+    uint32_t max_tokens;         /* rows of q and out, 1 .. 2^24 */
+    uint32_t max_new;            /* bound on one request's rows; 0: max_tokens */
+    uint32_t table_stride;       /* entries of a block_table row; times page_size at most 2^30 */
+    uint32_t window, sinks;      /* window 0: none */
+    float scale;                 /* 0: 1 / sqrt(head_dim) */
+    const void* q;               /* [max_tokens][heads * head_dim], 16-byte aligned */
+    void* out;                   /* as q; not q */
+    uint64_t q_stride, out_stride; /* elements between rows (0: packed); 16-byte multiples */
+    const uint32_t* query_start; /* [requests + 1], from 0 on and not decreasing */
+    const uint32_t* lens;        /* [requests] */
+    const uint32_t* block_table; /* [requests][table_stride] */
+} pk_hip_paged_attention;
+
+pk_hip_status pk_hip_paged_attention_async(pk_hip_ctx* ctx, const pk_hip_paged_attention* attention,
+                                           void* stream, char* error_buffer, size_t error_capacity);
 
 /* A plain streaming read of `bytes` device bytes at `src` on `stream`
  * (no counterpart in the reference: the measured floor of any kernel that

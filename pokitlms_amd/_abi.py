@@ -34,7 +34,8 @@ EXPORTS = (
     "pk_hip_weight_download", "pk_hip_moe_decode_noalloc", "pk_hip_dequantize_rows",
     "pk_hip_expf_block_sums", "pk_hip_rmsnorm", "pk_hip_add_rmsnorm", "pk_hip_matvec_add_rmsnorm", "pk_hip_attention_steps",
     "pk_hip_read_floor_async", "pk_hip_moe_decode_traced_async", "pk_hip_set_libm_expf",
-    "pk_hip_moe_decode_reference_order",
+    "pk_hip_moe_decode_reference_order", "pk_hip_paged_plan_async", "pk_hip_paged_append_async",
+    "pk_hip_paged_attention_async",
 )
 TRACE_WORDS = 3 * 8192 * 8
 
@@ -52,7 +53,9 @@ class Stats(ctypes.Structure):
         "gate_up_ns", "down_ns", "router_launches", "gate_up_launches", "down_launches",
         "matvec_launches", "prefill_calls", "prefill_tokens", "prefill_ns",
         "prefill_route_ns", "prefill_gate_up_ns", "prefill_down_ns", "q4_1_dispatches",
-        "q5_0_dispatches", "q5_1_dispatches", "q2_k_dispatches", "q3_k_dispatches")]
+        "q5_0_dispatches", "q5_1_dispatches", "q2_k_dispatches", "q3_k_dispatches",
+        "paged_plan_calls", "paged_append_calls", "paged_attention_calls", "paged_plan_ns",
+        "paged_append_ns", "paged_attention_ns")]
 
     def as_dict(self) -> dict:
         return {n: getattr(self, n) for n, _ in self._fields_}
@@ -95,6 +98,40 @@ class AttentionConfig(ctypes.Structure):
                 ("rms_eps", ctypes.c_float), ("rope_theta", ctypes.c_float),
                 ("reference_order", ctypes.c_uint32), ("libm_expf_pairs", ctypes.c_void_p),
                 ("libm_expf_count", ctypes.c_uint64)]
+
+
+class PagedKvDesc(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + [
+        (n, ctypes.c_uint32) for n in ("type", "pages", "page_size", "kv_heads", "head_dim")] + [
+        (n, ctypes.c_uint64) for n in ("page_stride", "slot_stride", "head_stride")]
+
+
+class PagedPlanDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in (
+        "requests", "pages", "page_size", "table_stride", "max_tokens")] + [
+        (n, ctypes.c_void_p) for n in (
+            "lens", "new_lens", "release", "block_table", "free_pages", "free_count", "lens_out",
+            "free_count_out", "query_start", "positions", "slots", "token_request", "status")]
+
+
+class PagedAppendDesc(ctypes.Structure):
+    _fields_ = [("cache", PagedKvDesc)] + [
+        (n, ctypes.c_uint32) for n in ("type", "tokens", "heads", "rotary_dim", "axes")] + [
+        ("rms_eps", ctypes.c_float), ("rope_theta", ctypes.c_float)] + [
+        (n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out")] + [
+        (n, ctypes.c_uint64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")] + [
+        (n, ctypes.c_void_p) for n in ("q_norm", "k_norm", "positions")] + [
+        ("position_stride", ctypes.c_uint64), ("pair_axis", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p)]
+
+
+class PagedAttentionDesc(ctypes.Structure):
+    _fields_ = [("cache", PagedKvDesc)] + [
+        (n, ctypes.c_uint32) for n in ("type", "heads", "requests", "max_tokens", "max_new",
+                                       "table_stride", "window", "sinks")] + [
+        ("scale", ctypes.c_float), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("q_stride", ctypes.c_uint64), ("out_stride", ctypes.c_uint64)] + [
+        (n, ctypes.c_void_p) for n in ("query_start", "lens", "block_table")]
 
 
 class GenerationStats(ctypes.Structure):
@@ -213,5 +250,11 @@ def lib() -> ctypes.CDLL:
                                            ctypes.POINTER(GenerationStats), cp, sz]
     L.pk_hip_synth_weight.restype = ctypes.c_int
     L.pk_hip_synth_weight.argtypes = [vp, u32, u64, u64, u32, u64, u32, ctypes.POINTER(vp), cp, sz]
+    for name, desc in (("pk_hip_paged_plan_async", PagedPlanDesc),
+                       ("pk_hip_paged_append_async", PagedAppendDesc),
+                       ("pk_hip_paged_attention_async", PagedAttentionDesc)):
+        f = getattr(L, name)
+        f.restype = ctypes.c_int
+        f.argtypes = [vp, ctypes.POINTER(desc), vp, cp, sz]
     _lib = L
     return L

@@ -132,6 +132,90 @@ class Moe35LayerHandles(MoeLayerHandles):
             w.release()
 
 
+class PagedKV:
+    """One layer's paged KV cache in device memory the caller owns (pk_hip_paged_kv):
+    k and v addresses, GGUF type (F16 or BF16), strides in elements (all 0: rows
+    packed as [page][slot][head])."""
+
+    def __init__(self, k: int, v: int, gtype: int, pages: int, page_size: int, kv_heads: int,
+                 head_dim: int, page_stride: int = 0, slot_stride: int = 0, head_stride: int = 0):
+        self.desc = _abi.PagedKvDesc(k, v, gtype, pages, page_size, kv_heads, head_dim,
+                                     page_stride, slot_stride, head_stride)
+
+
+class PagedPlan:
+    """The buffers of a step's plan (pk_hip_paged_plan): device addresses of uint32
+    arrays; built once, used for every step."""
+
+    def __init__(self, requests: int, pages: int, page_size: int, table_stride: int,
+                 max_tokens: int, *, lens: int, new_lens: int, block_table: int, free_pages: int,
+                 free_count: int, lens_out: int, free_count_out: int, query_start: int,
+                 positions: int, slots: int, token_request: int, status: int, release: int = 0):
+        self.desc = _abi.PagedPlanDesc(requests, pages, page_size, table_stride, max_tokens, lens,
+                                       new_lens, release or None, block_table, free_pages,
+                                       free_count, lens_out, free_count_out, query_start,
+                                       positions, slots, token_request, status)
+
+
+class PagedAppend:
+    """New tokens' rows on their way into a layer's cache (pk_hip_paged_append); strides
+    in elements (0: packed).  pair_axis: per rotated pair the row of positions it turns
+    by (None: row 0), e.g. from ``rotary_axes``."""
+
+    def __init__(self, cache: PagedKV, gtype: int, tokens: int, heads: int, *, k: int, v: int,
+                 slots: int, q: int = 0, q_out: int = 0, q_stride: int = 0, k_stride: int = 0,
+                 v_stride: int = 0, q_out_stride: int = 0, q_norm: int = 0, k_norm: int = 0,
+                 rms_eps: float = 0.0, rope_theta: float = 0.0, rotary_dim: int = 0,
+                 positions: int = 0, axes: int = 1, position_stride: int = 0, pair_axis=None):
+        axis = None
+        if pair_axis is not None:
+            if len(pair_axis) != rotary_dim // 2:
+                raise ValueError("pair_axis needs one axis per rotated pair")
+            if any(not 0 <= int(i) < 256 for i in pair_axis):
+                raise ValueError("pair_axis names an axis that is not there")
+            axis = (ctypes.c_uint8 * max(1, len(pair_axis)))(*[int(i) for i in pair_axis])
+        self.desc = _abi.PagedAppendDesc(
+            cache.desc, gtype, tokens, heads, rotary_dim, axes, rms_eps, rope_theta, q or None, k, v,
+            q_out or None, q_stride, k_stride, v_stride, q_out_stride, q_norm or None,
+            k_norm or None, positions or None, position_stride,
+            None if axis is None else ctypes.addressof(axis), slots)
+        self.desc.axis_map = axis  # lives as long as its address
+
+
+def rotary_axes(sections, interleaved: bool = False) -> list:
+    """The axis of each rotated pair for sections of pairs per axis, e.g. time, height and
+    width of an image or video: one section after the other, or, interleaved, the axes in
+    turn (0, 1, 2, 0, 1, 2, ..) for as long as those behind the first have pairs left, and
+    the first axis for the rest."""
+    sections = [int(n) for n in sections]
+    if not sections or any(n < 0 for n in sections):
+        raise ValueError("sections are counts of pairs")
+    if not interleaved:
+        return [axis for axis, n in enumerate(sections) for _ in range(n)]
+    out = [0] * sum(sections)
+    for axis in range(1, len(sections)):
+        at = range(axis, len(sections) * sections[axis], len(sections))
+        if len(at) != sections[axis] or (len(at) and at[-1] >= len(out)):
+            raise ValueError("sections do not interleave: the first axis has too few pairs")
+        for i in at:
+            out[i] = axis
+    return out
+
+
+class PagedAttention:
+    """New tokens' attention over a layer's cache (pk_hip_paged_attention); strides in
+    elements (0: packed), scale 0 for 1 / sqrt(head_dim), window 0 for none, max_new 0
+    for max_tokens."""
+
+    def __init__(self, cache: PagedKV, gtype: int, heads: int, requests: int, max_tokens: int, *,
+                 q: int, out: int, query_start: int, lens: int, block_table: int,
+                 table_stride: int, max_new: int = 0, window: int = 0, sinks: int = 0,
+                 scale: float = 0.0, q_stride: int = 0, out_stride: int = 0):
+        self.desc = _abi.PagedAttentionDesc(cache.desc, gtype, heads, requests, max_tokens, max_new,
+                                            table_stride, window, sinks, scale, q, out, q_stride,
+                                            out_stride, query_start, lens, block_table)
+
+
 class HipBackend:
     def __init__(self, device: int = 0, time_kernels: bool = False):
         L = _abi.lib()
@@ -492,6 +576,25 @@ class HipBackend:
                                                    device_x, tokens, device_y, device_ids,
                                                    device_probs, stream or None, err, _ERRBUF),
                err)
+
+    # ---- paged KV cache ---------------------------------------------------------------
+    def paged_plan_async(self, plan: PagedPlan, stream: int = 0) -> None:
+        """Pages, positions and slots of a step's new tokens (pk_hip_paged_plan_async)."""
+        err = ctypes.create_string_buffer(_ERRBUF)
+        _raise(_abi.lib().pk_hip_paged_plan_async(self.handle, ctypes.byref(plan.desc),
+                                                  stream or None, err, _ERRBUF), err)
+
+    def paged_append_async(self, append: PagedAppend, stream: int = 0) -> None:
+        """Head norms, rotation and K and V into the pages (pk_hip_paged_append_async)."""
+        err = ctypes.create_string_buffer(_ERRBUF)
+        _raise(_abi.lib().pk_hip_paged_append_async(self.handle, ctypes.byref(append.desc),
+                                                    stream or None, err, _ERRBUF), err)
+
+    def paged_attention_async(self, attention: PagedAttention, stream: int = 0) -> None:
+        """Attention of new tokens over the pages (pk_hip_paged_attention_async)."""
+        err = ctypes.create_string_buffer(_ERRBUF)
+        _raise(_abi.lib().pk_hip_paged_attention_async(self.handle, ctypes.byref(attention.desc),
+                                                       stream or None, err, _ERRBUF), err)
 
     def sync(self, stream: int = 0) -> None:
         err = ctypes.create_string_buffer(_ERRBUF)

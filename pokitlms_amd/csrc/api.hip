@@ -22,6 +22,7 @@
 #include "chunk_scratch.hpp"
 #include "launch.hpp"
 #include "layout.hpp"
+#include "paged_check.hpp"
 
 namespace {
 
@@ -180,6 +181,8 @@ struct pk_hip_ctx {
     DeviceBuffer<float> ref_scratch;
     DeviceBuffer<uint32_t> expf_slots;
     pk::LibmExpf expf{nullptr, 0, 0, 0};
+    // the paged cache's plans
+    DeviceBuffer<uint32_t> plan_work;
     hipEvent_t ev[10] = {};
     int wall_rate_khz = 100000;  // wall_clock64() rate
 
@@ -581,6 +584,29 @@ void sync_and_check(pk_hip_ctx* c, hipStream_t s) {
     }
 }
 
+void require(const pk::PagedCheck& c) {
+    if (!c.error) return;
+    if (c.unsupported) throw Unsupported(c.error);
+    throw ArgError(c.error);
+}
+
+// enqueue(stream) as an entry point's launches, timed into `ns` where launches are timed.
+template <typename F>
+void enqueue_paged(pk_hip_ctx* ctx, void* stream, uint64_t& calls, uint64_t& ns, F&& enqueue) {
+    ctx->set_device();
+    hipStream_t s = stream ? static_cast<hipStream_t>(stream) : ctx->stream;
+    const CaptureScope capture(s);
+    if (ctx->time_kernels) hold_stream(ctx, s);
+    begin_timing(ctx, s, 0);
+    enqueue(s);
+    begin_timing(ctx, s, 1);
+    ++calls;
+    if (ctx->time_kernels) {
+        check(hipStreamSynchronize(s), "hipStreamSynchronize");
+        ns += elapsed_ns(ctx, 0, 1);
+    }
+}
+
 }  // namespace
 
 extern "C" {
@@ -652,6 +678,7 @@ void pk_hip_destroy(pk_hip_ctx* c) {
     c->prow_bound.release();
     c->ref_scratch.release();
     c->expf_slots.release();
+    c->plan_work.release();
     for (auto& e : c->ev)
         if (e) (void)hipEventDestroy(e);
     if (c->stream) (void)hipStreamDestroy(c->stream);
@@ -2154,6 +2181,58 @@ pk_hip_status pk_hip_attention_steps(pk_hip_ctx* ctx, const pk_hip_attention_con
         sbuf.release();
         slots.release();
         kv.release();
+    });
+}
+
+// ---------------------------------------------------------------------------
+// The paged KV cache.
+
+pk_hip_status pk_hip_paged_plan_async(pk_hip_ctx* ctx, const pk_hip_paged_plan* plan, void* stream,
+                                      char* err, size_t cap) {
+    return guarded(ctx, err, cap, [&] {
+        pk::PagedPlanArgs a;
+        require(pk::check_plan(plan, a));
+        require_usable(ctx);
+        std::lock_guard lock(ctx->mutex);
+        enqueue_paged(ctx, stream, ctx->stats.paged_plan_calls, ctx->stats.paged_plan_ns, [&](hipStream_t s) {
+            const size_t words = pk::paged_plan_work_words(a.requests, a.max_tokens);
+            if (words) ctx->plan_work.ensure(words);
+            a.work = ctx->plan_work.ptr;
+            launch_checked(pk::launch_paged_plan(a, s), "paged plan launch");
+            ctx->stats.dispatches += words ? 2u : 1u;
+        });
+    });
+}
+
+pk_hip_status pk_hip_paged_append_async(pk_hip_ctx* ctx, const pk_hip_paged_append* append, void* stream,
+                                        char* err, size_t cap) {
+    return guarded(ctx, err, cap, [&] {
+        pk::PagedAppendArgs a;
+        require(pk::check_append(append, a));
+        require_usable(ctx);
+        std::lock_guard lock(ctx->mutex);
+        for (uint32_t i = 0; i < a.rotary_pairs; ++i)
+            a.turns[i] = std::pow(static_cast<double>(append->rope_theta), -static_cast<double>(i) / a.rotary_pairs) /
+                         6.283185307179586;
+        enqueue_paged(ctx, stream, ctx->stats.paged_append_calls, ctx->stats.paged_append_ns, [&](hipStream_t s) {
+            launch_checked(pk::launch_paged_append(a, s), "paged append launch");
+            ++ctx->stats.dispatches;
+        });
+    });
+}
+
+pk_hip_status pk_hip_paged_attention_async(pk_hip_ctx* ctx, const pk_hip_paged_attention* attention,
+                                           void* stream, char* err, size_t cap) {
+    return guarded(ctx, err, cap, [&] {
+        pk::PagedAttentionArgs a;
+        require(pk::check_attention(attention, a));
+        require_usable(ctx);
+        std::lock_guard lock(ctx->mutex);
+        enqueue_paged(ctx, stream, ctx->stats.paged_attention_calls, ctx->stats.paged_attention_ns,
+                      [&](hipStream_t s) {
+                          launch_checked(pk::launch_paged_attention(a, s), "paged attention launch");
+                          ++ctx->stats.dispatches;
+                      });
     });
 }
 

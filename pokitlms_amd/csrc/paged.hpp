@@ -1,0 +1,74 @@
+// paged.hpp -- host-side entry points of the paged KV cache's kernels (paged.hip,
+// paged_attention.hip): many requests share one pool of pages per layer.
+//
+// A request's position p lies in slot p % page_size of page table[p / page_size] of
+// its row of the block table.  A table entry that is not below `pages` is a page that
+// is not there: attention takes its positions as masked, append writes nothing.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace pk {
+
+constexpr uint32_t kNoSlot = 0xffffffffu;
+constexpr uint32_t kMaxPagedRequests = 8192;
+constexpr uint32_t kMaxPagedTokens = 1u << 24;  // rows of one call
+constexpr uint32_t kMaxPagedPositions = 1u << 30;  // positions a table row can hold
+constexpr uint32_t kMaxPageSize = 1024;
+
+struct PagedKv {
+    uint16_t *k, *v;          // row (page, slot, head) at their strides, in elements
+    uint32_t type;            // T_F16 or T_BF16
+    uint32_t pages, page_shift, kv_heads, head_dim;
+    uint64_t page_stride, slot_stride, head_stride;
+};
+
+// Plan: see pk_hip_paged_plan in pokit_hip.h.  work: 2 * requests + 1 words of scratch
+// where the plan takes two launches (plan_work_words).
+struct PagedPlanArgs {
+    uint32_t requests, page_shift, pages, table_stride, max_tokens;
+    const uint32_t *lens, *new_lens, *release, *free_count;
+    uint32_t *table, *free_pages;
+    uint32_t *lens_out, *free_count_out, *query_start, *positions, *slots, *token_request, *status;
+    uint32_t* work;
+};
+size_t paged_plan_work_words(uint32_t requests, uint32_t max_tokens);
+hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t stream);
+
+// Append: head norms, rotation and the store into the pages (pk_hip_paged_append).
+constexpr uint32_t kMaxRotaryPairs = 128;
+constexpr uint32_t kMaxRotaryAxes = 4;
+struct PagedAppendArgs {
+    PagedKv kv;
+    uint32_t type;            // of q, k, v and q_out: T_F32, T_F16 or T_BF16
+    uint32_t tokens, heads, rotary_pairs, axes;
+    float eps;
+    const void *q, *k, *v;
+    void* q_out;
+    uint64_t q_stride, k_stride, v_stride, q_out_stride;  // elements between tokens' rows
+    const float *q_norm, *k_norm;                         // [head_dim], or null: no norm
+    const uint32_t* positions;                            // [axes][position_stride]
+    uint64_t position_stride;
+    const uint32_t* slots;
+    double turns[kMaxRotaryPairs];    // theta^(-i / pairs) / 2 pi
+    uint8_t axis[kMaxRotaryPairs];
+};
+hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t stream);
+
+// Attention over the pages (pk_hip_paged_attention).
+struct PagedAttentionArgs {
+    PagedKv kv;
+    uint32_t type;            // of q and out
+    uint32_t heads, group;    // group = heads / kv_heads
+    uint32_t requests, max_tokens, max_new, table_stride;
+    const void* q;
+    void* out;
+    uint64_t q_stride, out_stride;  // elements between tokens' rows
+    const uint32_t *query_start, *lens, *table;
+    float scale;
+    uint32_t window, sinks;   // window 0: none
+};
+hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t stream);
+
+}  // namespace pk
