@@ -181,8 +181,9 @@ struct pk_hip_ctx {
     DeviceBuffer<float> ref_scratch;
     DeviceBuffer<uint32_t> expf_slots;
     pk::LibmExpf expf{nullptr, 0, 0, 0};
-    // the paged cache's plans
+    // the paged cache's plans, and the parts of its attention's long rows
     DeviceBuffer<uint32_t> plan_work;
+    DeviceBuffer<float> attn_work;
     hipEvent_t ev[10] = {};
     int wall_rate_khz = 100000;  // wall_clock64() rate
 
@@ -679,6 +680,7 @@ void pk_hip_destroy(pk_hip_ctx* c) {
     c->ref_scratch.release();
     c->expf_slots.release();
     c->plan_work.release();
+    c->attn_work.release();
     for (auto& e : c->ev)
         if (e) (void)hipEventDestroy(e);
     if (c->stream) (void)hipStreamDestroy(c->stream);
@@ -2230,7 +2232,10 @@ pk_hip_status pk_hip_paged_attention_async(pk_hip_ctx* ctx, const pk_hip_paged_a
         std::lock_guard lock(ctx->mutex);
         enqueue_paged(ctx, stream, ctx->stats.paged_attention_calls, ctx->stats.paged_attention_ns,
                       [&](hipStream_t s) {
-                          launch_checked(pk::launch_paged_attention(a, s), "paged attention launch");
+                          const size_t floats = pk::paged_attention_work_floats(a);
+                          if (floats) ctx->attn_work.ensure(floats);
+                          launch_checked(pk::launch_paged_attention(a, ctx->attn_work.ptr, s),
+                                         "paged attention launch");
                           ++ctx->stats.dispatches;
                       });
     });

@@ -69,6 +69,8 @@ struct PagedAttentionArgs {
     float scale;
     uint32_t window, sinks;   // window 0: none
 };
-hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t stream);
+// work: paged_attention_work_floats(a) floats of scratch, 16-byte aligned.
+size_t paged_attention_work_floats(const PagedAttentionArgs& a);
+hipError_t launch_paged_attention(const PagedAttentionArgs& a, float* work, hipStream_t stream);
 
 }  // namespace pk

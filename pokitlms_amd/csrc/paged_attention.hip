@@ -4,79 +4,909 @@
 // position i of its request's pages if i <= p, its page is there, and, with a window W,
 // i + W > p or i < sinks.  Head h reads kv head h / group:
 //   o = sum_i softmax_i(scale * q . k_i) v_i, and 0 where nothing is seen.
+//
+// One pass over K and V with a running maximum m and sum l per row (in units of log 2):
+// o <- o * 2^(m - m') + sum_i 2^(c s_i - m') v_i, with c = scale * log2(e).  Rows of one
+// kv head's query heads share a tile, so K and V are read once for all of them.  Both
+// products run on the matrix cores as S^T = K Q^T and O^T = V^T P^T: a lane then holds
+// scores of one row only, maximum, sum and rescaling stay in the lane (and the few that
+// share its row), and the weights are in the layout that the second product takes, with
+// the keys of a tile in the order in which the first left them.
+//
+// FP32 rows enter the 16-bit products as parts, q = q0 + q1 (+ q2) and likewise the weights:
+// two F16 parts hold 22 bits (q under a power of two per row, weights times 2^12, so that
+// small ones keep them), three BF16 parts 24.  16-bit rows round the weights once to
+// the cache's type, half a step of the output's own rounding.
 #include <hip/hip_fp16.h>
 #include <math.h>
 
 #include "kquant.hpp"
 #include "paged.hpp"
+#include "paged_index.hpp"
 
 namespace pk {
 namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <uint32_t T> struct Mat;
+template <> struct Mat<T_F16> {
+    using E = _Float16;
+    typedef _Float16 V8 __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x4 mma16(V8 a, V8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mma32(V8 a, V8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct Mat<T_BF16> {
+    using E = __bf16;
+    typedef __bf16 V8 __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x4 mma16(V8 a, V8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mma32(V8 a, V8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
+constexpr uint32_t parts_of(uint32_t T, bool f32) { return !f32 ? 1u : T == T_F16 ? 2u : 3u; }
+
+// The maximum moves (and o and l are rescaled) only when it has grown by 2^3; weights are
+// at most 2^(kBias + 3), inside F16.
+constexpr float kBias = 12.0f, kSlack = 3.0f;
+
+// 8 values as NP parts: v = parts[0] + parts[1] + ...
+template <typename M, uint32_t NP>
+__device__ __forceinline__ void split8(const float* v, typename M::V8* parts) {
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) {
+        float rest = v[e];
+#pragma unroll
+        for (uint32_t i = 0; i < NP; ++i) {
+            const auto h = static_cast<typename M::E>(rest);
+            parts[i][e] = h;
+            rest -= static_cast<float>(h);
+        }
+    }
+}
 
 __device__ __forceinline__ float cache_value(uint32_t type, uint16_t bits) {
     return type == T_F16 ? half_bits_to_float(bits) : __uint_as_float(static_cast<uint32_t>(bits) << 16);
 }
 
-// One wave per (token, head): 64 positions at a time, a score per lane, then the values
-// with a running maximum and sum.
-__global__ __launch_bounds__(64) void k_paged_attention_plain(PagedAttentionArgs a) {
-    __shared__ float q[256];
-    const uint32_t t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, HD = a.kv.head_dim;
-    uint32_t r = a.requests;
-    for (uint32_t i = 0; i < a.requests; ++i)
-        if (a.query_start[i] <= t && t < a.query_start[i + 1u]) r = i;
-    if (r == a.requests || a.query_start[r + 1u] - a.query_start[r] > a.max_new) return;
-    const int64_t len = a.lens[r], p = len - (a.query_start[r + 1u] - t);
-    const uint64_t at = t * a.q_stride + h * HD;
-    for (uint32_t d = lane; d < HD; d += 64u)
-        q[d] = a.scale * (a.type == T_F32 ? static_cast<const float*>(a.q)[at + d]
-                                          : cache_value(a.type, static_cast<const uint16_t*>(a.q)[at + d]));
-    __syncthreads();
+// A launch's share of the rows, and its scratch: parts of split tiles (BM rows of head_dim
+// sums, then their m and l), for each its tile if it is the tile's first, and their number.
+struct RowWork {
+    uint32_t min_rows, max_rows, target, least;
+    float* part;
+    uint32_t* head;   // [most_parts][4]: parts (0: not the first), request, tile, kv head
+    uint32_t* count;  // [1]
+};
+
+// One workgroup's piece: part `part` of `parts` of row tile `tile` of request r.
+struct Piece {
+    uint32_t r, q0, fresh, tile, part, parts, slot;
+    int32_t len;
+};
+
+// The piece of unit u, from the lengths alone: every wave finds it by itself (64 requests
+// at a time, one per lane; exclusive sums give each request its units).  total: parts of
+// split tiles per kv head.
+__device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, const RowWork& w, uint32_t bm, uint32_t u,
+                                           Piece& p, uint32_t& total) {
+    const uint32_t lane = threadIdx.x & 63u, per = (a.requests + 63u) / 64u;
+    const uint32_t positions = a.table_stride << a.kv.page_shift;
+    auto work_of = [&](uint32_t r) -> RequestWork {
+        if (r >= a.requests) return {0u, 0u};
+        const uint32_t fresh = paged_new(a.query_start[r], a.query_start[r + 1u], a.max_new, a.max_tokens);
+        return request_work(fresh, a.lens[r], a.group, bm, w.min_rows, w.max_rows, a.window, a.sinks, positions);
+    };
+    RequestWork one{0u, 0u};  // per == 1: the lane's request
+    uint64_t work = 0;
+    for (uint32_t i = 0; i < per; ++i) {
+        one = work_of(lane * per + i);
+        work += static_cast<uint64_t>(one.tiles) * one.keys;
+    }
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d *= 2) work += __shfl_xor(work, d);
+    const uint64_t pieces = part_pieces(work * a.kv.kv_heads, w.target, w.least);
+    uint32_t units = 0u, slots = 0u;
+    for (uint32_t i = 0; i < per; ++i) {
+        if (per > 1u) one = work_of(lane * per + i);
+        const uint32_t n = request_parts(one.keys, pieces);
+        units += one.tiles * n;
+        slots += n > 1u ? one.tiles * n : 0u;
+    }
+    uint32_t eu = units, es = slots;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d *= 2) {
+        const uint32_t x = __shfl_up(eu, d), y = __shfl_up(es, d);
+        eu += lane >= d ? x : 0u;
+        es += lane >= d ? y : 0u;
+    }
+    total = __builtin_amdgcn_readlane(es, 63);
+    eu -= units;
+    es -= slots;
+    const uint64_t mine = __ballot(u >= eu && u - eu < units);
+    if (!mine) return false;
+    uint32_t r = lane * per, left = u - eu;
+    for (uint32_t i = 0; i < per; ++i) {  // only the owner's walk matters
+        if (per > 1u) one = work_of(lane * per + i);
+        const uint32_t n = request_parts(one.keys, pieces);
+        r = lane * per + i;
+        if (left < one.tiles * n || i + 1u == per) break;
+        left -= one.tiles * n;
+        es += n > 1u ? one.tiles * n : 0u;
+    }
+    const int owner = __builtin_ctzll(mine);
+    auto get = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), owner)); };
+    const uint32_t tiles = get(one.tiles), at = get(left);
+    p.r = get(r);
+    p.parts = request_parts(get(one.keys), pieces);
+    p.tile = tiles - 1u - at / p.parts;  // the tiles that see most keys first
+    p.part = at % p.parts;
+    p.slot = get(es) + at;
+    p.q0 = a.query_start[p.r];
+    p.fresh = a.query_start[p.r + 1u] - p.q0;
+    p.len = static_cast<int32_t>(a.lens[p.r] < positions ? a.lens[p.r] : positions);
+    return true;
+}
+
+// 4 values of a row of q's type.
+__device__ __forceinline__ void store4(uint32_t type, void* out, uint64_t at, f32x4 v) {
+    if (type == T_F32) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at) = v;
+    } else if (type == T_F16) {
+        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<h4*>(static_cast<uint16_t*>(out) + at) = __builtin_convertvector(v, h4);
+    } else {
+        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<b4*>(static_cast<uint16_t*>(out) + at) = __builtin_convertvector(v, b4);
+    }
+}
+
+// Where a row's result goes: its output, or its place among the parts.
+struct RowTo {
+    void* out;
+    uint64_t at;
+    float* part;  // [HD] sums, or null
+    float* ml;
+};
+__device__ __forceinline__ RowTo row_to(const PagedAttentionArgs& a, const RowWork& w, const Piece& p, uint32_t bm,
+                                        uint32_t hk, uint32_t row) {
+    const uint32_t f = p.tile * bm + row, HD = a.kv.head_dim;
+    RowTo to{a.out, (p.q0 + f / a.group) * a.out_stride + (hk * a.group + f % a.group) * HD, nullptr, nullptr};
+    if (p.parts > 1u) {
+        float* base = w.part + static_cast<uint64_t>(p.slot * a.kv.kv_heads + hk) * bm * (HD + 2u);
+        to.part = base + row * HD;
+        to.ml = base + bm * HD + 2u * row;
+    }
+    return to;
+}
+__device__ __forceinline__ void store_row4(const PagedAttentionArgs& a, const RowTo& to, uint32_t d, f32x4 o, float m,
+                                           float l) {
+    if (to.part) {
+        *reinterpret_cast<f32x4*>(to.part + d) = o;
+        if (d == 0u) {
+            to.ml[0] = m;
+            to.ml[1] = l;
+        }
+    } else {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        store4(a.type, to.out, to.at + d, f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv});
+    }
+}
+
+// The split tile's head word, written by its first part.
+__device__ __forceinline__ void write_head(const PagedAttentionArgs& a, const RowWork& w, const Piece& p, uint32_t hk) {
+    if (p.parts == 1u) return;
+    uint32_t* h = w.head + 4u * (p.slot * a.kv.kv_heads + hk);
+    h[0] = p.part == 0u ? p.parts : 0u;
+    h[1] = p.r;
+    h[2] = p.tile;
+    h[3] = hk;
+}
+
+// One row over the key tiles t0 .. t1 - 1 by one wave, reading only what the row sees: for
+// rows into which a masked value (NaN or infinite, with weight 0) has come by way of a
+// tile whose other rows see it.
+__device__ void row_alone(const PagedAttentionArgs& a, const Piece& p, const KeyTiles& keys, uint32_t kt, uint32_t t0,
+                          uint32_t t1, uint32_t hk, uint32_t f, const RowTo& to) {
+    const uint32_t lane = threadIdx.x & 63u, HD = a.kv.head_dim, token = p.q0 + f / a.group;
+    const int32_t pos = p.len - static_cast<int32_t>(p.fresh) + static_cast<int32_t>(f / a.group);
+    const uint64_t at = token * a.q_stride + (hk * a.group + f % a.group) * HD;
+    const float c = a.scale * 1.4426950408889634f;
     const uint32_t mask = (1u << a.kv.page_shift) - 1u;
-    const int64_t cap = static_cast<int64_t>(a.table_stride) << a.kv.page_shift;
-    float m = -INFINITY, sum = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t i0 = 0; i0 <= p && i0 < cap; i0 += 64) {
-        const int64_t i = i0 + lane;
-        bool seen = i <= p && i < cap && (a.window == 0u || i + a.window > p || i < a.sinks);
-        const uint32_t page = seen ? a.table[static_cast<uint64_t>(r) * a.table_stride + (i >> a.kv.page_shift)] : kNoSlot;
-        seen = page < a.kv.pages;
-        const uint64_t row = seen ? page * a.kv.page_stride + (i & mask) * a.kv.slot_stride + (h / a.group) * a.kv.head_stride : 0u;
+    const uint32_t* table = a.table + static_cast<uint64_t>(p.r) * a.table_stride;
+    float m = -INFINITY, l = 0.0f;
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t t = t0; t < t1; ++t) {
+        const uint32_t i = keys.base(t, kt) + lane;
+        uint32_t page = kNoSlot;
+        if (lane < kt && row_sees(pos, i, a.window, a.sinks) && (i >> a.kv.page_shift) < a.table_stride)
+            page = table[i >> a.kv.page_shift];
+        const bool seen = page < a.kv.pages;
+        const uint64_t row = seen ? page * a.kv.page_stride + (i & mask) * a.kv.slot_stride + hk * a.kv.head_stride : 0u;
         float s = -INFINITY;
         if (seen) {
             s = 0.0f;
-            for (uint32_t d = 0; d < HD; ++d) s = fmaf(q[d], cache_value(a.kv.type, a.kv.k[row + d]), s);
+            for (uint32_t d = 0; d < HD; ++d) {
+                const float q = a.type == T_F32 ? static_cast<const float*>(a.q)[at + d]
+                                                : cache_value(a.type, static_cast<const uint16_t*>(a.q)[at + d]);
+                s = fmaf(q, cache_value(a.kv.type, a.kv.k[row + d]), s);
+            }
+            s *= c;
         }
         float top = s;
-        for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-        if (top == -INFINITY) continue;
-        const float next = fmaxf(m, top), e = seen ? expf(s - next) : 0.0f, keep = expf(m - next);
+        for (uint32_t d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+        if (!__any(seen)) continue;
+        const float next = fmaxf(m, top), ref = next == -INFINITY ? 0.0f : next;
+        const float e = seen ? exp2f(s - ref) : 0.0f, keep = exp2f(m - ref);
         float es = e;
-        for (int d = 32; d > 0; d >>= 1) es += __shfl_xor(es, d);
-        sum = sum * keep + es;
-        for (uint32_t c = 0; c < HD / 64u; ++c) o[c] *= keep;
-        for (uint32_t l = 0; l < 64u; ++l) {
-            const float w = __shfl(e, l);
-            const uint64_t vr = __shfl(row, l);
-            if (w == 0.0f) continue;
-            for (uint32_t c = 0; c < HD / 64u; ++c) o[c] = fmaf(w, cache_value(a.kv.type, a.kv.v[vr + 64u * c + lane]), o[c]);
+        for (uint32_t d = 32; d > 0; d >>= 1) es += __shfl_xor(es, d);
+        l = l * keep + es;
+        for (uint32_t k = 0; k < 4u; ++k) o[k] *= keep;
+        for (uint32_t j = 0; j < kt; ++j) {
+            const float x = __shfl(e, j);
+            const uint64_t vr = __shfl(row, j);
+            if (x == 0.0f) continue;
+            for (uint32_t k = 0; k < 4u; ++k)
+                if (4u * lane + k < HD) o[k] = fmaf(x, cache_value(a.kv.type, a.kv.v[vr + 4u * lane + k]), o[k]);
         }
         m = next;
     }
-    const uint64_t to = t * a.out_stride + h * HD;
-    for (uint32_t c = 0; c < HD / 64u; ++c) {
-        const float v = sum > 0.0f ? o[c] / sum : 0.0f;
-        const uint64_t d = to + 64u * c + lane;
-        if (a.type == T_F32) static_cast<float*>(a.out)[d] = v;
-        else if (a.type == T_F16) static_cast<_Float16*>(a.out)[d] = static_cast<_Float16>(v);
-        else static_cast<__bf16*>(a.out)[d] = static_cast<__bf16>(v);
+    // the other rows' sums are 2^kBias times as large under the same m
+    if (4u * lane < HD) store_row4(a, to, 4u * lane, f32x4{o[0], o[1], o[2], o[3]}, m + kBias, l);
+}
+
+__device__ __forceinline__ float max_over(float v, uint32_t d) { return fmaxf(v, __shfl_xor(v, d)); }
+
+// A lane's part of its row: 8 values at q + at + STEP * k of each k, as parts.  F16 parts of
+// FP32 rows come under a power of two, which goes to c; the row's other lanes are MIN, 2 MIN ..
+// lanes away.
+template <uint32_t T, bool F32, uint32_t KK, uint32_t STEP, uint32_t MIN>
+__device__ __forceinline__ void load_q(const PagedAttentionArgs& a, uint64_t at, bool live,
+                                       typename Mat<T>::V8 (*q)[KK], float& c) {
+    using M = Mat<T>;
+    constexpr uint32_t NP = parts_of(T, F32);
+    if constexpr (!F32) {
+#pragma unroll
+        for (uint32_t k = 0; k < KK; ++k) {
+            u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at + STEP * k);
+            if (!live) x = u32x4{0u, 0u, 0u, 0u};
+            q[0][k] = __builtin_bit_cast(typename M::V8, x);
+        }
+    } else {
+        float v[KK][8], top = 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < KK; ++k) {
+            const f32x4* src = reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + at + STEP * k);
+            const f32x4 x = src[0], y = src[1];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                v[k][e] = !live ? 0.0f : e < 4u ? x[e & 3u] : y[e & 3u];
+                top = fmaxf(top, fabsf(v[k][e]));
+            }
+        }
+        if constexpr (T == T_F16) {
+#pragma unroll
+            for (uint32_t d = MIN; d < 64u; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+            // the largest value to [2^14, 2^15)
+            const int ex = top > 0.0f && top < INFINITY ? static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14 : 0;
+            const float up = ldexpf(1.0f, -ex / 2), up2 = ldexpf(1.0f, -ex - (-ex / 2));
+#pragma unroll
+            for (uint32_t k = 0; k < KK; ++k)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) v[k][e] = v[k][e] * up * up2;
+            c = fmaxf(ldexpf(c, ex), 1.1754944e-38f);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < KK; ++k) {
+            typename M::V8 part[NP];
+            split8<M, NP>(v[k], part);
+#pragma unroll
+            for (uint32_t i = 0; i < NP; ++i) q[i][k] = part[i];
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows (single tokens): one tile of 16 rows, four waves that take the tile's keys in
+// turn, 32 at a time, straight from memory into the matrix operands.
+//
+// K rows are the first product's A operand as they lie (8 values of a row per lane).  V is
+// the second product's A operand transposed, a value of 8 rows per lane: a lane loads the
+// same HD / 16 columns of 8 rows and exchanges halves of its own registers, and column
+// (l % 16) * HD / 16 + e is row l % 16 of product e.  Reading K and V bounds it: the next
+// K is on its way while the weights are taken, the next V while the next scores are.
+template <uint32_t T, uint32_t HD, bool F32>
+__global__ __launch_bounds__(256) void k_paged_rows(PagedAttentionArgs a, RowWork w) {
+    using M = Mat<T>;
+    using V8 = typename M::V8;
+    constexpr uint32_t NP = parts_of(T, F32), KK = HD / 32u, DPL = HD / 16u, BM = 16u, KT = 32u, PITCH = HD + 4u;
+    __shared__ __attribute__((aligned(16))) uint64_t s_off[4][KT];
+    __shared__ __attribute__((aligned(16))) float s_o[4][BM][PITCH];
+    __shared__ float s_m[4][BM], s_l[4][BM];
+    __shared__ uint32_t s_bad;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, g = lane >> 4, j = lane & 15u;
+    const uint32_t hk = blockIdx.x % a.kv.kv_heads;
+    Piece p;
+    uint32_t total;
+    const bool live_piece = find_piece(a, w, BM, blockIdx.x / a.kv.kv_heads, p, total);
+    if (w.count && blockIdx.x == 0u && tid == 0u) w.count[0] = total * a.kv.kv_heads;
+    if (!live_piece) return;
+    if (tid == 0u) {
+        write_head(a, w, p, hk);
+        s_bad = 0u;
+    }
+    const uint32_t rows = p.fresh * a.group - p.tile * BM < BM ? p.fresh * a.group - p.tile * BM : BM;
+    const uint32_t positions = a.table_stride << a.kv.page_shift, mask = (1u << a.kv.page_shift) - 1u;
+    const int32_t p0 = p.len - static_cast<int32_t>(p.fresh);
+    const int32_t p_first = p0 + static_cast<int32_t>(p.tile * BM / a.group);
+    const int32_t p_last = p0 + static_cast<int32_t>((p.tile * BM + rows - 1u) / a.group);
+    const KeyTiles keys = key_tiles(p_first, p_last, a.window, a.sinks, positions, KT);
+    uint32_t b0, b1;
+    part_range(keys.tiles, p.part, p.parts, b0, b1);
+    // this lane's row: q parts and position
+    const uint32_t f = p.tile * BM + j;
+    const bool live = j < rows;
+    const int32_t pos = live ? p0 + static_cast<int32_t>(f / a.group) : -1;
+    V8 q[NP][KK];
+    float c = a.scale * 1.4426950408889634f;
+    load_q<T, F32, KK, 32u, 16u>(a, (p.q0 + (live ? f / a.group : 0u)) * a.q_stride +
+                                    (hk * a.group + (live ? f % a.group : 0u)) * HD + 8u * g, live, q, c);
+    const uint32_t* table = a.table + static_cast<uint64_t>(p.r) * a.table_stride;
+    const uint16_t* kbase = a.kv.k + hk * a.kv.head_stride + 8u * g;
+    const uint16_t* vbase = a.kv.v + hk * a.kv.head_stride + DPL * j;
+    const uint32_t lo = a.window && p_first >= 0 && static_cast<uint32_t>(p_first) + 1u > a.window
+                            ? static_cast<uint32_t>(p_first) + 1u - a.window : 0u;
+    // the table entry of position base(b) + lane % 32, where any row may see it
+    auto entry = [&](uint32_t b) -> uint32_t {
+        const uint32_t i = keys.base(b, KT) + (lane & 31u);
+        const bool in = static_cast<int32_t>(i) <= p_last && i < positions && (i >= lo || i < a.sinks);
+        return in ? table[i >> a.kv.page_shift] : kNoSlot;
+    };
+    uint32_t there = 0u;
+    auto place = [&](uint32_t b, uint32_t page) {
+        const uint32_t i = keys.base(b, KT) + (lane & 31u);
+        const bool in = page < a.kv.pages;
+        there = static_cast<uint32_t>(__ballot(in));
+        s_off[wave][lane & 31u] = in ? page * a.kv.page_stride + (i & mask) * a.kv.slot_stride : 0u;
+        __builtin_amdgcn_wave_barrier();
+    };
+    u32x4 kr[2][KK];
+    constexpr uint32_t VW = DPL / 2u;  // dwords of a V row per lane
+    uint32_t vr[8][VW];
+    auto load_k = [&] {
+#pragma unroll
+        for (uint32_t t = 0; t < 2; ++t) {
+            const uint16_t* src = kbase + s_off[wave][16u * t + j];
+#pragma unroll
+            for (uint32_t k = 0; k < KK; ++k) kr[t][k] = *reinterpret_cast<const u32x4*>(src + 32u * k);
+        }
+    };
+    auto load_v = [&] {
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+            const uint16_t* src = vbase + s_off[wave][16u * (e / 4u) + 4u * g + e % 4u];
+            if constexpr (VW == 2u) {
+                const u32x2 x = *reinterpret_cast<const u32x2*>(src);
+                vr[e][0] = x[0];
+                vr[e][1] = x[1];
+            } else {
+#pragma unroll
+                for (uint32_t h = 0; h < VW / 4u; ++h) {
+                    const u32x4 x = reinterpret_cast<const u32x4*>(src)[h];
+#pragma unroll
+                    for (uint32_t y = 0; y < 4; ++y) vr[e][4u * h + y] = x[y];
+                }
+            }
+        }
+    };
+    f32x4 o[DPL];
+#pragma unroll
+    for (uint32_t e = 0; e < DPL; ++e) o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    uint32_t b = b0 + wave, next_page = kNoSlot;
+    if (b < b1) {
+        place(b, entry(b));
+        load_k();
+        load_v();
+        if (b + 4u < b1) next_page = entry(b + 4u);
+    }
+    for (; b < b1; b += 4u) {
+        const uint32_t base = keys.base(b, KT), here = there;
+        f32x4 s[2];
+#pragma unroll
+        for (uint32_t t = 0; t < 2; ++t) {
+            s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (uint32_t k = 0; k < KK; ++k)
+#pragma unroll
+                for (uint32_t i = 0; i < NP; ++i) s[t] = M::mma16(__builtin_bit_cast(V8, kr[t][k]), q[i][k], s[t]);
+        }
+        const bool more = b + 4u < b1;
+        if (more) {
+            place(b + 4u, next_page);
+            load_k();
+            if (b + 8u < b1) next_page = entry(b + 8u);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // every row sees the whole tile, or each score asks
+        if (here != 0xffffffffu || static_cast<int32_t>(base + KT) - 1 > p_first ||
+            (a.window && base + a.window <= static_cast<uint32_t>(p_last) && base + KT > a.sinks)) {
+#pragma unroll
+            for (uint32_t t = 0; t < 2; ++t)
+#pragma unroll
+                for (uint32_t x = 0; x < 4; ++x) {
+                    const uint32_t at = 16u * t + 4u * g + x;
+                    if (!((here >> at) & 1u) || !row_sees(pos, base + at, a.window, a.sinks)) s[t][x] = -INFINITY;
+                }
+            if (here != 0xffffffffu)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e)
+                    if (!((here >> (16u * (e / 4u) + 4u * g + e % 4u)) & 1u))
+#pragma unroll
+                        for (uint32_t y = 0; y < VW; ++y) vr[e][y] = 0u;
+        }
+        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        top = max_over(max_over(top, 16u), 32u) * c;
+        if (__any(top > m + kSlack)) {
+            const float mm = fmaxf(m, top), keep = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mm);
+            m = mm;
+            l *= keep;
+#pragma unroll
+            for (uint32_t e = 0; e < DPL; ++e) o[e] = o[e] * keep;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m - kBias;
+        float pw[8];
+#pragma unroll
+        for (uint32_t x = 0; x < 8; ++x) {
+            pw[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x / 4u][x % 4u], c, -ref));
+            l += pw[x];
+        }
+        V8 pp[NP];
+        split8<M, NP>(pw, pp);
+#pragma unroll
+        for (uint32_t e = 0; e < DPL; ++e) {
+            u32x4 x;
+#pragma unroll
+            for (uint32_t y = 0; y < 4; ++y)
+                x[y] = __builtin_amdgcn_perm(vr[2u * y + 1u][e / 2u], vr[2u * y][e / 2u],
+                                             e % 2u ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (uint32_t i = 0; i < NP; ++i) o[e] = M::mma16(__builtin_bit_cast(V8, x), pp[i], o[e]);
+        }
+        if (more) load_v();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // the four waves' parts
+    l += __shfl_xor(l, 16u);
+    l += __shfl_xor(l, 32u);
+    if (g == 0u) {
+        s_m[wave][j] = m;
+        s_l[wave][j] = l;
+    }
+    __syncthreads();
+    {
+        const float mm = fmaxf(fmaxf(s_m[0][j], s_m[1][j]), fmaxf(s_m[2][j], s_m[3][j]));
+        const float keep = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mm);
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x)
+#pragma unroll
+            for (uint32_t e = 0; e < DPL; e += 4)
+                *reinterpret_cast<f32x4*>(&s_o[wave][j][(4u * g + x) * DPL + e]) =
+                    f32x4{o[e][x] * keep, o[e + 1][x] * keep, o[e + 2][x] * keep, o[e + 3][x] * keep};
+    }
+    __syncthreads();
+    const uint32_t row = tid / 16u;
+    const float mm = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+    float sum = 0.0f;
+#pragma unroll
+    for (uint32_t v = 0; v < 4; ++v) sum += mm == -INFINITY ? s_l[v][row] : s_l[v][row] * __builtin_amdgcn_exp2f(s_m[v][row] - mm);
+    f32x4 r[HD / 64u];
+    bool bad = false;
+#pragma unroll
+    for (uint32_t k = 0; k < HD / 64u; ++k) {
+        const uint32_t d = 64u * k + 4u * (tid % 16u);
+        r[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (uint32_t v = 0; v < 4; ++v) r[k] = r[k] + *reinterpret_cast<const f32x4*>(&s_o[v][row][d]);
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x) bad = bad || r[k][x] != r[k][x];
+    }
+    if (bad && row < rows) atomicOr(&s_bad, 1u << row);
+    __syncthreads();
+    const uint32_t again = p_first != p_last ? s_bad : 0u;
+    if (row < rows && !((again >> row) & 1u)) {
+        const RowTo to = row_to(a, w, p, BM, hk, row);
+#pragma unroll
+        for (uint32_t k = 0; k < HD / 64u; ++k) store_row4(a, to, 64u * k + 4u * (tid % 16u), r[k], mm, sum);
+    }
+    if (again)
+        for (uint32_t i = wave; i < rows; i += 4u)
+            if ((again >> i) & 1u) row_alone(a, p, keys, KT, b0, b1, hk, p.tile * BM + i, row_to(a, w, p, BM, hk, i));
+}
+
+// ---------------------------------------------------------------------------
+// Many rows (chunks of prompts): tiles of 128 rows, 32 per wave, over tiles of 64 keys that
+// all four waves read from LDS, two tiles of K and V in turn: one is read while the other's
+// loads go straight into LDS.  A row of a tile is HD / 8 pieces of 16 bytes; piece c of row r
+// lies at c ^ swizzle(r), so that neither the 32 rows that the first product reads side by
+// side nor the 4 rows by 32 columns of the transposing reads of the second meet in a bank.
+constexpr uint32_t kTileRows = 128u, kTileKeys = 64u;
+
+template <uint32_t HD>
+__device__ __forceinline__ uint32_t swizzle(uint32_t r) {
+    return HD == 64u ? (((r >> 1) & 1u) << 2) | ((r >> 2) & 3u) : ((r & 3u) << 2) | ((r >> 2) & 3u);
+}
+
+// What a row that is not there is read from.
+__device__ __attribute__((aligned(16))) uint16_t g_no_row[256];
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
+typedef uint8_t __attribute__((address_space(3))) * lds_ptr;
+
+// 16 bytes per lane from src into LDS, lane after lane from `to` (the same for all lanes).
+// Written out, since the builtin makes every later LDS read wait for it: the loop waits
+// itself, once per tile, before the barrier that lets the tile be read.
+__device__ __forceinline__ void load_to_lds(const void* src, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(to) : "memory", "m0");
+}
+
+template <uint32_t T, uint32_t HD, bool F32>
+__global__ __launch_bounds__(256, HD <= 128u && !F32 ? 2 : 1) void k_paged_tiles(PagedAttentionArgs a, RowWork w) {
+    using M = Mat<T>;
+    using V8 = typename M::V8;
+    constexpr uint32_t NP = parts_of(T, F32), KK = HD / 16u, DT = HD / 32u, BM = kTileRows, KT = kTileKeys;
+    constexpr uint32_t ROWB = 2u * HD, CH = HD / 8u, RPI = 1024u / ROWB, NI = KT / RPI / 4u;
+    __shared__ __attribute__((aligned(1024))) uint8_t s_k[2][KT * ROWB], s_v[2][KT * ROWB];
+    __shared__ uint32_t s_gone[2][4];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t h = lane >> 5, j = lane & 31u, hk = blockIdx.x % a.kv.kv_heads;
+    Piece p;
+    uint32_t total;
+    const bool live_piece = find_piece(a, w, BM, blockIdx.x / a.kv.kv_heads, p, total);
+    if (w.count && blockIdx.x == 0u && tid == 0u) w.count[0] = total * a.kv.kv_heads;
+    if (!live_piece) return;
+    if (tid == 0u) write_head(a, w, p, hk);
+    const uint32_t left = p.fresh * a.group - p.tile * BM, rows = left < BM ? left : BM;
+    const uint32_t positions = a.table_stride << a.kv.page_shift, mask = (1u << a.kv.page_shift) - 1u;
+    const int32_t p0 = p.len - static_cast<int32_t>(p.fresh);
+    const int32_t p_first = p0 + static_cast<int32_t>(p.tile * BM / a.group);
+    const int32_t p_last = p0 + static_cast<int32_t>((p.tile * BM + rows - 1u) / a.group);
+    const KeyTiles keys = key_tiles(p_first, p_last, a.window, a.sinks, positions, KT);
+    uint32_t t0, t1;
+    part_range(keys.tiles, p.part, p.parts, t0, t1);
+    const uint32_t lo = a.window && p_first >= 0 && static_cast<uint32_t>(p_first) + 1u > a.window
+                            ? static_cast<uint32_t>(p_first) + 1u - a.window : 0u;
+    // this wave's rows and this lane's
+    const uint32_t f0 = p.tile * BM + 32u * wave, f = f0 + j;
+    const bool live = 32u * wave + j < rows, wave_live = 32u * wave < rows;
+    const uint32_t wrows = wave_live ? (rows - 32u * wave < 32u ? rows - 32u * wave : 32u) : 0u;
+    const int32_t w_first = p0 + static_cast<int32_t>(f0 / a.group);
+    const int32_t w_last = wave_live ? p0 + static_cast<int32_t>((f0 + wrows - 1u) / a.group) : -1;
+    const int32_t pos = live ? p0 + static_cast<int32_t>(f / a.group) : -1;
+    V8 q[NP][KK];
+    float c = a.scale * 1.4426950408889634f;
+    load_q<T, F32, KK, 16u, 32u>(a, (p.q0 + (live ? f / a.group : 0u)) * a.q_stride +
+                                    (hk * a.group + (live ? f % a.group : 0u)) * HD + 8u * h, live, q, c);
+    // loads: this lane's row of each of the wave's NI pieces of a tile, 16 bytes of it
+    const uint32_t* table = a.table + static_cast<uint64_t>(p.r) * a.table_stride;
+    const uint32_t in_row = lane / CH;
+    const uint32_t lds_k = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)&s_k[0][0]));
+    const uint32_t lds_v = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)&s_v[0][0]));
+    uint32_t page[NI];
+    auto entries = [&](uint32_t t) {
+        const uint32_t base = keys.base(t, KT);
+#pragma unroll
+        for (uint32_t n = 0; n < NI; ++n) {
+            const uint32_t i = base + (wave * NI + n) * RPI + in_row;
+            const bool in = static_cast<int32_t>(i) <= p_last && i < positions && (i >= lo || i < a.sinks);
+            page[n] = in ? table[i >> a.kv.page_shift] : kNoSlot;
+        }
+    };
+    auto load = [&](uint32_t t, uint32_t buf) {
+        const uint32_t base = keys.base(t, KT);
+        bool gone = false;
+#pragma unroll
+        for (uint32_t n = 0; n < NI; ++n) {
+            const uint32_t row = (wave * NI + n) * RPI + in_row, i = base + row;
+            const uint32_t piece = 8u * ((lane % CH) ^ swizzle<HD>(row));
+            const bool in = page[n] < a.kv.pages;
+            gone = gone || (!in && static_cast<int32_t>(i) <= p_last && (i >= lo || i < a.sinks));
+            const uint64_t off = page[n] * a.kv.page_stride + (i & mask) * a.kv.slot_stride + hk * a.kv.head_stride;
+            const uint16_t* ks = in ? a.kv.k + off : g_no_row;
+            const uint16_t* vs = in ? a.kv.v + off : g_no_row;
+            const uint32_t to = buf * KT * ROWB + (wave * NI + n) * 1024u;
+            load_to_lds(ks + piece, __builtin_amdgcn_readfirstlane(lds_k + to));
+            load_to_lds(vs + piece, __builtin_amdgcn_readfirstlane(lds_v + to));
+        }
+        const bool any = __any(gone);
+        if (lane == 0u) s_gone[buf][wave] = any;
+    };
+    // where this lane reads: K row j, its piece 2 k + h; V rows 4 h + 8 second + (lane % 16) / 4,
+    // columns 32 dt + 16 ((lane / 16) % 2) + 4 (lane % 4)
+    const uint32_t kf = swizzle<HD>(j) ^ h;
+    uint32_t vat[2][DT];
+#pragma unroll
+    for (uint32_t second = 0; second < 2; ++second)
+#pragma unroll
+        for (uint32_t dt = 0; dt < DT; ++dt) {
+            const uint32_t row = 4u * h + 8u * second + (lane & 15u) / 4u;
+            const uint32_t piece = 4u * dt + 2u * ((lane >> 4) & 1u) + (lane & 3u) / 2u;
+            vat[second][dt] = row * ROWB + 16u * (piece ^ swizzle<HD>(row)) + 8u * (lane & 1u);
+        }
+    f32x16 o[DT];
+#pragma unroll
+    for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+        for (uint32_t x = 0; x < 16; ++x) o[d][x] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    if (t0 < t1) {
+        entries(t0);
+        load(t0, 0u);
+        if (t0 + 1u < t1) entries(t0 + 1u);
+    }
+    for (uint32_t t = t0; t < t1; ++t) {
+        const uint32_t buf = (t - t0) & 1u, base = keys.base(t, KT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of the tile have landed
+        __syncthreads();                                  // and everyone's; the other buffer has been read
+        if (t + 1u < t1) {
+            load(t + 1u, buf ^ 1u);
+            if (t + 2u < t1) entries(t + 2u);
+        }
+        // nothing of the tile for this wave's rows
+        if (static_cast<int32_t>(base) > w_last ||
+            (a.window && w_first >= 0 && base + (KT - 1u) + a.window <= static_cast<uint32_t>(w_first) && base >= a.sinks))
+            continue;
+        f32x16 s[2];
+#pragma unroll
+        for (uint32_t ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (uint32_t x = 0; x < 16; ++x) s[ks][x] = 0.0f;
+        const uint8_t* kb = s_k[buf] + j * ROWB;
+#pragma unroll
+        for (uint32_t k = 0; k < KK; ++k)
+#pragma unroll
+            for (uint32_t ks = 0; ks < 2; ++ks) {
+                const V8 x = *reinterpret_cast<const V8*>(kb + 32u * ks * ROWB + 16u * (kf ^ (2u * k)));
+#pragma unroll
+                for (uint32_t i = 0; i < NP; ++i) s[ks] = M::mma32(x, q[i][k], s[ks]);
+            }
+        const uint32_t gone = s_gone[buf][0] | s_gone[buf][1] | s_gone[buf][2] | s_gone[buf][3];
+        if (gone || static_cast<int32_t>(base + KT) - 1 > w_first ||
+            (a.window && base + a.window <= static_cast<uint32_t>(w_last) && base + KT > a.sinks)) {
+#pragma unroll
+            for (uint32_t ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (uint32_t x = 0; x < 16; ++x) {
+                    const uint32_t i = base + 32u * ks + 8u * (x / 4u) + 4u * h + x % 4u;
+                    bool seen = row_sees(pos, i, a.window, a.sinks) && i < positions;
+                    if (gone && seen) seen = table[i >> a.kv.page_shift] < a.kv.pages;
+                    if (!seen) s[ks][x] = -INFINITY;
+                }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (uint32_t ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (uint32_t x = 0; x < 16; ++x) top = fmaxf(top, s[ks][x]);
+        top = max_over(top, 32u) * c;
+        if (__any(top > m + kSlack)) {
+            const float mm = fmaxf(m, top), keep = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mm);
+            m = mm;
+            l *= keep;
+#pragma unroll
+            for (uint32_t d = 0; d < DT; ++d) o[d] = o[d] * keep;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m - kBias;
+#pragma unroll
+        for (uint32_t ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (uint32_t t16 = 0; t16 < 2; ++t16) {
+                float pw[8];
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) {
+                    pw[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[ks][8u * t16 + e], c, -ref));
+                    l += pw[e];
+                }
+                V8 pp[NP];
+                split8<M, NP>(pw, pp);
+#pragma unroll
+                for (uint32_t d = 0; d < DT; ++d) {
+                    struct { s16x4 a, b; } x;
+                    uint8_t* vb = s_v[buf] + (32u * ks + 16u * t16) * ROWB;
+                    x.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(vb + vat[0][d]));
+                    x.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(vb + vat[1][d]));
+#pragma unroll
+                    for (uint32_t i = 0; i < NP; ++i) o[d] = M::mma32(__builtin_bit_cast(V8, x), pp[i], o[d]);
+                }
+            }
+    }
+    if (!wave_live) return;
+    l += __shfl_xor(l, 32u);
+    bool bad = false;
+#pragma unroll
+    for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+        for (uint32_t x = 0; x < 16; ++x) bad = bad || o[d][x] != o[d][x];
+    uint64_t again = w_first != w_last ? __ballot(bad && live) : 0u;
+    again = (again | (again >> 32)) & 0xffffffffu;
+    if (live && !((again >> j) & 1u)) {
+        const RowTo to = row_to(a, w, p, BM, hk, 32u * wave + j);
+#pragma unroll
+        for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+            for (uint32_t x = 0; x < 16; x += 4)
+                store_row4(a, to, 32u * d + 2u * x + 4u * h, f32x4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]}, m, l);
+    }
+    while (again) {
+        const uint32_t i = static_cast<uint32_t>(__builtin_ctzll(again));
+        again &= again - 1u;
+        row_alone(a, p, keys, KT, t0, t1, hk, f0 + i, row_to(a, w, p, BM, hk, 32u * wave + i));
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Joins the parts of split tiles.  WG (slot, y): if the slot is its tile's first part, rows
+// y * RPW .. of it: HD / 4 lanes a row, SPLIT: the rest of the workgroup over the parts, else
+// over the rows.
+template <uint32_t HD, uint32_t BM, uint32_t RPW, bool SPLIT>
+__global__ __launch_bounds__(256) void k_paged_join(PagedAttentionArgs a, RowWork w) {
+    constexpr uint32_t LANES = HD / 4u, GROUPS = 256u / LANES;
+    static_assert(!SPLIT || RPW == 1u);
+    __shared__ __attribute__((aligned(16))) float s_o[SPLIT ? GROUPS : 1u][HD];
+    __shared__ float s_m[SPLIT ? GROUPS : 1u], s_l[SPLIT ? GROUPS : 1u];
+    const uint32_t slot = blockIdx.x, tid = threadIdx.x, lane = tid % LANES, grp = tid / LANES;
+    if (slot >= w.count[0]) return;
+    const uint32_t* h = w.head + 4u * slot;
+    const uint32_t parts = h[0];
+    if (parts == 0u) return;
+    Piece p{};
+    p.r = h[1];
+    p.tile = h[2];
+    p.parts = 1u;
+    p.q0 = a.query_start[p.r];
+    p.fresh = a.query_start[p.r + 1u] - p.q0;
+    const uint32_t left = p.fresh * a.group - p.tile * BM, rows = left < BM ? left : BM;
+    const uint64_t stride = static_cast<uint64_t>(a.kv.kv_heads) * BM * (HD + 2u);
+    const float* base = w.part + static_cast<uint64_t>(slot) * BM * (HD + 2u);
+    for (uint32_t row = blockIdx.y * RPW + (SPLIT ? 0u : grp); row < blockIdx.y * RPW + RPW && row < rows;
+         row += SPLIT ? 1u : GROUPS) {
+        float m = -INFINITY, l = 0.0f;
+        f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t i = SPLIT ? grp : 0u; i < parts; i += SPLIT ? GROUPS : 1u) {
+            const float* at = base + i * stride;
+            const f32x4 x = *reinterpret_cast<const f32x4*>(at + row * HD + 4u * lane);
+            const float pm = at[BM * HD + 2u * row], pl = at[BM * HD + 2u * row + 1u];
+            const float mm = fmaxf(m, pm);
+            if (mm == -INFINITY) {  // nothing seen yet, or NaN alone
+                l += pl;
+                o = o + x;
+                continue;
+            }
+            const float k0 = __builtin_amdgcn_exp2f(m - mm), k1 = __builtin_amdgcn_exp2f(pm - mm);
+            o = o * k0 + x * k1;
+            l = l * k0 + pl * k1;
+            m = mm;
+        }
+        if constexpr (SPLIT) {
+            *reinterpret_cast<f32x4*>(&s_o[grp][4u * lane]) = o;
+            if (lane == 0u) {
+                s_m[grp] = m;
+                s_l[grp] = l;
+            }
+            __syncthreads();
+            if (grp == 0u) {
+                float mm = -INFINITY;
+                for (uint32_t i = 0; i < GROUPS; ++i) mm = fmaxf(mm, s_m[i]);
+                l = 0.0f;
+                o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (uint32_t i = 0; i < GROUPS; ++i) {
+                    const float k = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s_m[i] - mm);
+                    o = o + *reinterpret_cast<const f32x4*>(&s_o[i][4u * lane]) * k;
+                    l += s_l[i] * k;
+                }
+                m = mm;
+            }
+        }
+        if (!SPLIT || grp == 0u) store_row4(a, row_to(a, w, p, BM, h[3], row), 4u * lane, o, m, l);
+    }
+}
+
+// Rows of a request (new tokens times group) up to which the 16-row tiles take it.
+constexpr uint32_t kFewRows = 32u;
+// Workgroups that a launch spreads split tiles over, and a part's least work in
+// kScheduleKeys positions.
+constexpr uint32_t kRowsTarget = 1024u, kRowsLeast = 4u, kTilesTarget = 512u, kTilesLeast = 8u;
+
+bool may_split(const PagedAttentionArgs& a, uint32_t least) {
+    const uint64_t positions = static_cast<uint64_t>(a.table_stride) << a.kv.page_shift;
+    return positions / kScheduleKeys + 2u > least + least / 4u;
+}
+
+// One of the two launches of a call, its scratch and what it needs of it.
+struct Half {
+    RowWork w;
+    uint32_t bm;
+    bool used, splits;
+    uint64_t part_floats() const { return splits ? most_parts(w.target) * bm : 0u; }
+    uint64_t words() const { return splits ? most_parts(w.target) * 4u + 4u : 0u; }
+};
+void halves(const PagedAttentionArgs& a, Half& few, Half& many) {
+    few = Half{{1u, kFewRows, kRowsTarget, kRowsLeast, nullptr, nullptr, nullptr}, 16u, a.group <= kFewRows,
+               may_split(a, kRowsLeast)};
+    many = Half{{kFewRows + 1u, 0xffffffffu, kTilesTarget, kTilesLeast, nullptr, nullptr, nullptr}, kTileRows,
+                static_cast<uint64_t>(a.max_new) * a.group > kFewRows, may_split(a, kTilesLeast)};
+    few.splits = few.splits && few.used;
+    many.splits = many.splits && many.used;
+}
+
+template <uint32_t T, uint32_t HD, bool F32>
+hipError_t attention_t(const PagedAttentionArgs& a, const Half& few, const Half& many, hipStream_t s) {
+    const uint32_t kvh = a.kv.kv_heads;
+    const dim3 b(256);
+    // a call of single tokens has at most kFewRows rows of each of min(requests, tokens) requests
+    const uint64_t n = a.requests < a.max_tokens ? a.requests : a.max_tokens;
+    const uint64_t few_tokens = n * (kFewRows / a.group ? kFewRows / a.group : 1u);
+    const uint64_t fu = most_units(most_tiles(few_tokens < a.max_tokens ? few_tokens : a.max_tokens, a.requests, a.group,
+                                              few.bm), kvh, few.splits ? few.w.target : 0u) * kvh;
+    const uint64_t mu = most_units(most_tiles(a.max_tokens, a.requests, a.group, many.bm), kvh,
+                                   many.splits ? many.w.target : 0u) * kvh;
+    if (fu >= (1ull << 31) || mu >= (1ull << 31)) return hipErrorInvalidValue;
+    if (many.used)
+        hipLaunchKernelGGL((k_paged_tiles<T, HD, F32>), dim3(static_cast<uint32_t>(mu)), b, 0, s, a, many.w);
+    if (few.used)
+        hipLaunchKernelGGL((k_paged_rows<T, HD, F32>), dim3(static_cast<uint32_t>(fu)), b, 0, s, a, few.w);
+    if (many.splits)
+        hipLaunchKernelGGL((k_paged_join<HD, kTileRows, 16, false>), dim3(most_parts(many.w.target), kTileRows / 16u), b, 0,
+                           s, a, many.w);
+    if (few.splits)
+        hipLaunchKernelGGL((k_paged_join<HD, 16, 1, true>), dim3(most_parts(few.w.target), 16), b, 0, s, a, few.w);
+    return hipGetLastError();
+}
+
+template <uint32_t T, bool F32>
+hipError_t attention_hd(const PagedAttentionArgs& a, const Half& few, const Half& many, hipStream_t s) {
+    switch (a.kv.head_dim) {
+        case 64: return attention_t<T, 64, F32>(a, few, many, s);
+        case 128: return attention_t<T, 128, F32>(a, few, many, s);
+        case 256: return attention_t<T, 256, F32>(a, few, many, s);
+        default: return hipErrorInvalidValue;
     }
 }
 
 }  // namespace
 
-hipError_t launch_paged_attention(const PagedAttentionArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL(k_paged_attention_plain, dim3(a.max_tokens, a.heads), dim3(64), 0, s, a);
-    return hipGetLastError();
+size_t paged_attention_work_floats(const PagedAttentionArgs& a) {
+    Half few, many;
+    halves(a, few, many);
+    return (few.part_floats() + many.part_floats()) * (a.kv.head_dim + 2u) + few.words() + many.words();
+}
+
+hipError_t launch_paged_attention(const PagedAttentionArgs& a, float* work, hipStream_t s) {
+    Half few, many;
+    halves(a, few, many);
+    float* at = work;
+    for (Half* half : {&few, &many}) {
+        if (!half->splits) continue;
+        half->w.part = at;
+        at += half->part_floats() * (a.kv.head_dim + 2u);
+        half->w.head = reinterpret_cast<uint32_t*>(at);
+        half->w.count = half->w.head + most_parts(half->w.target) * 4u;
+        at += half->words();
+    }
+    const bool f32 = a.type == T_F32;
+    if (a.kv.type == T_F16) return f32 ? attention_hd<T_F16, true>(a, few, many, s) : attention_hd<T_F16, false>(a, few, many, s);
+    return f32 ? attention_hd<T_BF16, true>(a, few, many, s) : attention_hd<T_BF16, false>(a, few, many, s);
 }
 
 }  // namespace pk

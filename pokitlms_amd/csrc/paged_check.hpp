@@ -166,6 +166,8 @@ inline PagedCheck check_attention(const pk_hip_paged_attention* p, PagedAttentio
     if (p->heads == 0u || p->heads > 4096u || p->heads % p->cache.kv_heads)
         return {"query heads must be evenly grouped over KV heads"};
     if (p->max_tokens == 0u || p->max_tokens > kMaxPagedTokens) return {"max_tokens must be between 1 and 2^24"};
+    if (static_cast<uint64_t>(p->max_tokens) * p->heads >= (1ull << 31))
+        return {"max_tokens times heads must be below 2^31"};
     if (!p->q || !p->out || !p->query_start || !p->lens || !p->block_table)
         return {"q, out, query_start, lens and block_table are required"};
     if (!aligned16(p->q) || !aligned16(p->out)) return {"rows must be 16-byte aligned"};

@@ -1,0 +1,113 @@
+// The paged attention's index arithmetic (csrc/paged_index.hpp) against plain loops, on the
+// host: which keys a tile visits, how a launch's work is cut, and that neither workgroups
+// nor scratch are ever short.  Prints "ok" and the number of cases.
+#include <cstdio>
+#include <cstdlib>
+#include <vector>
+
+#include "../../pokitlms_amd/csrc/paged_index.hpp"
+
+namespace {
+
+uint64_t state = 1;
+uint32_t draw(uint32_t n) {
+    state = state * 6364136223846793005ull + 1442695040888963407ull;
+    return static_cast<uint32_t>((state >> 33) % n);
+}
+
+#define CHECK(x)                                                        \
+    do {                                                                \
+        if (!(x)) {                                                     \
+            std::printf("line %d: %s (case %u)\n", __LINE__, #x, at);   \
+            std::exit(1);                                               \
+        }                                                               \
+    } while (0)
+
+// Every position that a row of the tile sees is visited once, in order, below `positions`
+// rounded up to a tile; no tile lies outside [0, p_last].
+void keys(uint32_t at) {
+    const uint32_t kt = draw(2) ? 32 : 64, positions = 1 + draw(600);
+    const int32_t p_first = static_cast<int32_t>(draw(650)) - 40, p_last = p_first + static_cast<int32_t>(draw(40));
+    const uint32_t window = draw(2) ? 0 : 1 + draw(300), sinks = draw(2) ? draw(5) : draw(400);
+    const pk::KeyTiles t = pk::key_tiles(p_first, p_last, window, sinks, positions, kt);
+    std::vector<int> seen(positions + kt, 0);
+    uint32_t last = 0;
+    for (uint32_t i = 0; i < t.tiles; ++i) {
+        const uint32_t base = t.base(i, kt);
+        CHECK(base % kt == 0 && base < positions && static_cast<int32_t>(base) <= p_last);
+        CHECK(i == 0 || base > last);
+        last = base;
+        for (uint32_t k = 0; k < kt; ++k) ++seen[base + k];
+    }
+    for (int32_t p = p_first; p <= p_last; ++p)
+        for (uint32_t i = 0; i < positions; ++i) {
+            const bool want = p >= 0 && static_cast<int64_t>(i) <= p &&
+                              (!window || static_cast<int64_t>(i) + window > p || i < sinks);
+            CHECK(pk::row_sees(p, i, window, sinks) == want);
+            if (want) CHECK(seen[i] == 1);
+        }
+    // the parts of a tile are its tiles in order, each once
+    const uint32_t parts = 1 + draw(9);
+    uint32_t next = 0;
+    for (uint32_t i = 0; i < parts; ++i) {
+        uint32_t t0, t1;
+        pk::part_range(t.tiles, i, parts, t0, t1);
+        CHECK(t0 == next && t1 >= t0 && t1 <= t.tiles);
+        next = t1;
+    }
+    CHECK(next == t.tiles);
+}
+
+void schedule(uint32_t at) {
+    const uint32_t bm = draw(2) ? 16 : 128, group = 1 + draw(draw(2) ? 9 : 70), kv_heads = 1 + draw(8);
+    const uint32_t target = 1u << draw(11), least = 1 + draw(8), requests = 1 + draw(40);
+    const uint32_t min_rows = draw(2) ? 1 : 33, max_rows = draw(2) ? 32 : 0xffffffffu;
+    const uint32_t window = draw(3) ? 0 : 1 + draw(3000), sinks = draw(200), positions = 64 + draw(40000);
+    const uint32_t tokens = 1 + draw(3000), max_new = 1 + draw(tokens);
+    std::vector<uint32_t> start(requests + 1, 0), lens(requests);
+    for (uint32_t r = 0; r < requests; ++r) {
+        uint32_t n = draw(3) ? draw(3) : draw(1 + draw(800));
+        if (start[r] + n > tokens) n = tokens - start[r];
+        start[r + 1] = start[r] + n;
+        lens[r] = draw(4) ? draw(positions + 1) : draw(0x80000000u);  // beyond the table too
+    }
+    uint64_t work = 0;
+    std::vector<pk::RequestWork> all;
+    for (uint32_t r = 0; r < requests; ++r) {
+        const uint32_t fresh = pk::paged_new(start[r], start[r + 1], max_new, tokens);
+        CHECK(fresh == (start[r + 1] - start[r] > max_new ? 0 : start[r + 1] - start[r]));
+        all.push_back(pk::request_work(fresh, lens[r], group, bm, min_rows, max_rows, window, sinks, positions));
+        const uint64_t rows = uint64_t(fresh) * group;
+        CHECK(all[r].tiles == (rows >= min_rows && rows <= max_rows ? (rows + bm - 1) / bm : 0));
+        work += uint64_t(all[r].tiles) * all[r].keys;
+    }
+    const uint64_t pieces = pk::part_pieces(work * kv_heads, target, least);
+    uint64_t units = 0, parts = 0;
+    for (const pk::RequestWork& r : all) {
+        const uint32_t n = pk::request_parts(r.keys, pieces);
+        CHECK(n >= 1);
+        units += uint64_t(r.tiles) * n;
+        if (n > 1) parts += uint64_t(r.tiles) * n;
+    }
+    CHECK(units <= pk::most_units(pk::most_tiles(tokens, requests, group, bm), kv_heads, target));
+    CHECK(parts * kv_heads <= pk::most_parts(target));
+    // a cache whose rows are too short to be split has no parts
+    if (positions / pk::kScheduleKeys + 2 <= least + least / 4) CHECK(parts == 0);
+}
+
+void bad_lengths(uint32_t at) {
+    const uint32_t q0 = draw(100), q1 = draw(100), most = 1 + draw(100), tokens = 1 + draw(100);
+    const uint32_t n = pk::paged_new(q0, q1, most, tokens);
+    CHECK(n <= most && (n == 0 || (q0 + n == q1 && q1 <= tokens)));
+}
+
+}  // namespace
+
+int main() {
+    uint32_t at = 0;
+    for (; at < 3000; ++at) keys(at);
+    for (; at < 60000; ++at) schedule(at);
+    for (; at < 80000; ++at) bad_lengths(at);
+    std::printf("ok %u\n", at);
+    return 0;
+}

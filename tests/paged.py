@@ -80,18 +80,19 @@ def attention(q, k, v, table, start, lens, page, scale, window, sinks):
         n, new = int(lens[r]), int(start[r + 1]) - int(start[r])
         for j in range(new):
             t, p = int(start[r]) + j, n - new + j
-            seen = [i for i in range(p + 1) if (not window or i + window > p or i < sinks)
-                    and i // page < table.shape[1] and table[r, i // page] < pages]
-            at = [int(table[r, i // page]) for i in seen], [i % page for i in seen]
+            i = np.arange(min(p + 1, table.shape[1] * page))
+            seen = (i + window > p) | (i < sinks) if window else np.ones(len(i), bool)
+            i = i[seen & (table[r, i // page] < pages)]
+            at = table[r, i // page].astype(np.int64), i % page
             for a in range(h):
                 out[t, a] = 0.0
-                if not seen:
+                if not len(i):
                     continue
                 kk, vv = k[at[0], at[1], a // (h // kvh)], v[at[0], at[1], a // (h // kvh)]
                 s = scale * (kk @ q[t, a])
                 w = np.exp(s - s.max())
                 out[t, a] = (w / w.sum()) @ vv
-                bound[t, a] = scale * np.abs(kk * q[t, a]).sum(-1).max(), np.abs(vv).max(), len(seen)
+                bound[t, a] = scale * np.abs(kk * q[t, a]).sum(-1).max(), np.abs(vv).max(), len(i)
     return out, bound
 
 

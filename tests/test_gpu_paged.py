@@ -453,6 +453,45 @@ def test_attention_drawn(hip, seed):
     check_attention(c, run_attention(hip, c, window=window, sinks=sinks), window, sinks)
 
 
+@pytest.mark.parametrize("gtype,cache,dim", [("F32", "F16", 64), ("F16", "F16", 128), ("F32", "BF16", 128),
+                                             ("BF16", "BF16", 256)])
+@pytest.mark.parametrize("new", ([1, 1, 1], [40, 1, 3], [90, 130, 20]))
+@pytest.mark.parametrize("window,sinks", [(0, 0), (3000, 5), (100, 2500)])
+def test_attention_long_contexts(hip, gtype, cache, dim, new, window, sinks):
+    """Rows whose keys are spread over several workgroups and joined."""
+    c = attention_case(dim + sum(new), [9001, 700, 5003], new, 4, 2, dim, gtype, cache, 16, width_more=900)
+    check_attention(c, run_attention(hip, c, window=window, sinks=sinks), window, sinks)
+
+
+def test_attention_masked_values_in_long_contexts(hip):
+    """A later token's NaN and infinity, in the part of the keys that holds the rows themselves."""
+    for new in ([4, 1], [60, 1]):
+        c = attention_case(31, [6000, 100], new, 8, 2, 128, "F32", "F16", 16)
+        page = int(c["table"][0, 5999 // 16])
+        c["v"][page, 5999 % 16], c["v"][page, 5998 % 16, 0, 3] = float("nan"), float("inf")
+        got = run_attention(hip, c)
+        clean = {**c, "v": c["v"].nan_to_num(0, 0, 0)}
+        ref = run_attention(hip, clean)
+        n = new[0]
+        want, bound = P.attention(f64(c["q"]), f64(clean["k"]), f64(clean["v"]), c["table"], c["start"], c["lens"],
+                                  16, 128 ** -0.5, 0, 0)
+        tol = P.attention_tolerance(np.nan_to_num(want), bound, 128, "F32", "F16")
+        rows = list(range(n - 2)) + [n]
+        assert np.all(np.abs(f64(got) - want)[rows] <= tol[rows])
+        assert torch.isnan(got[n - 1]).all() and torch.all(got[n - 2, :4, 3] == float("inf"))
+        assert torch.equal(got[n - 2, 4:], ref[n - 2, 4:]) or np.all(
+            np.abs(f64(got) - want)[n - 2, 4:] <= tol[n - 2, 4:])
+
+
+@pytest.mark.parametrize("requests", (65, 200, 1030))
+def test_attention_many_requests(hip, requests):
+    g = np.random.default_rng(requests)
+    lens, new = P.ragged(g, requests, 90, 2)
+    lens[7], new[7] = 400, 70
+    c = attention_case(requests, lens, new, 2, 1, 64, "F16", "F16", 8)
+    check_attention(c, run_attention(hip, c))
+
+
 def test_attention_order_does_not_change_bits(hip):
     c = attention_case(13, [3000, 700], [1, 1], 8, 2, 128, "F32", "F16", 16)
     first = run_attention(hip, c)
