@@ -225,6 +225,10 @@ class HipBackend:
         _raise(L.pk_hip_create(device, ctypes.byref(opts), ctypes.byref(h), err, _ERRBUF), err)
         self.handle = h.value
         self._cache = {}
+        # the paged calls come many times a step: their functions and error text are kept
+        self._err = ctypes.create_string_buffer(_ERRBUF)
+        self._plan, self._append = L.pk_hip_paged_plan_async, L.pk_hip_paged_append_async
+        self._attend = L.pk_hip_paged_attention_async
 
     # ---- lifetime ---------------------------------------------------------------
     def close(self) -> None:
@@ -580,21 +584,21 @@ class HipBackend:
     # ---- paged KV cache ---------------------------------------------------------------
     def paged_plan_async(self, plan: PagedPlan, stream: int = 0) -> None:
         """Pages, positions and slots of a step's new tokens (pk_hip_paged_plan_async)."""
-        err = ctypes.create_string_buffer(_ERRBUF)
-        _raise(_abi.lib().pk_hip_paged_plan_async(self.handle, ctypes.byref(plan.desc),
-                                                  stream or None, err, _ERRBUF), err)
+        status = self._plan(self.handle, plan.desc, stream or None, self._err, _ERRBUF)
+        if status:
+            _raise(status, self._err)
 
     def paged_append_async(self, append: PagedAppend, stream: int = 0) -> None:
         """Head norms, rotation and K and V into the pages (pk_hip_paged_append_async)."""
-        err = ctypes.create_string_buffer(_ERRBUF)
-        _raise(_abi.lib().pk_hip_paged_append_async(self.handle, ctypes.byref(append.desc),
-                                                    stream or None, err, _ERRBUF), err)
+        status = self._append(self.handle, append.desc, stream or None, self._err, _ERRBUF)
+        if status:
+            _raise(status, self._err)
 
     def paged_attention_async(self, attention: PagedAttention, stream: int = 0) -> None:
         """Attention of new tokens over the pages (pk_hip_paged_attention_async)."""
-        err = ctypes.create_string_buffer(_ERRBUF)
-        _raise(_abi.lib().pk_hip_paged_attention_async(self.handle, ctypes.byref(attention.desc),
-                                                       stream or None, err, _ERRBUF), err)
+        status = self._attend(self.handle, attention.desc, stream or None, self._err, _ERRBUF)
+        if status:
+            _raise(status, self._err)
 
     def sync(self, stream: int = 0) -> None:
         err = ctypes.create_string_buffer(_ERRBUF)

@@ -30,21 +30,23 @@ constexpr uint32_t kPlanThreads = 1024;
 constexpr uint32_t kPlanFusedTokens = 4096;
 
 struct PlanSums {
-    uint64_t tokens;
-    uint32_t need, back;
+    uint32_t tokens, need, back;
 };
 
-__device__ __forceinline__ PlanSums wave_scan(PlanSums v, uint32_t lane) {
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d *= 2) {
-        const uint64_t t = __shfl_up(v.tokens, d);
-        const uint32_t n = __shfl_up(v.need, d), b = __shfl_up(v.back, d);
-        if (lane >= d) {
-            v.tokens += t;
-            v.need += n;
-            v.back += b;
-        }
-    }
+// Inclusive sums over the lanes.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ void scan_step(PlanSums& v) {
+    v.tokens += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v.tokens), CTRL, ROWS, 0xf, false));
+    v.need += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v.need), CTRL, ROWS, 0xf, false));
+    v.back += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v.back), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ PlanSums wave_scan(PlanSums v) {
+    scan_step<0x111>(v);
+    scan_step<0x112>(v);
+    scan_step<0x114>(v);
+    scan_step<0x118>(v);
+    scan_step<0x142, 0xa>(v);
+    scan_step<0x143, 0xc>(v);
     return v;
 }
 
@@ -156,7 +158,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PagedPlanArgs a) {
         mine.need += need[i];
         mine.back += rel[i];
     }
-    PlanSums at = wave_scan(mine, lane);
+    // a sum past max_tokens only has to stay past it
+    if (mine.tokens > kMaxPagedTokens + 1u) mine.tokens = kMaxPagedTokens + 1u;
+    PlanSums at = wave_scan(mine);
     if (lane == 63u) wave_total[wave] = at;
     at.tokens -= mine.tokens;
     at.need -= mine.need;
@@ -164,6 +168,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PagedPlanArgs a) {
     if (flags) atomicOr(&bad, flags);
     __syncthreads();
     PlanSums total{0, 0, 0};
+    uint64_t tokens_sum = 0;
 #pragma unroll
     for (uint32_t w = 0; w < kPlanThreads / 64; ++w) {
         const PlanSums s = wave_total[w];
@@ -172,15 +177,15 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PagedPlanArgs a) {
             at.need += s.need;
             at.back += s.back;
         }
-        total.tokens += s.tokens;
+        tokens_sum += s.tokens;
         total.need += s.need;
         total.back += s.back;
     }
     flags = bad;
     if (count > a.pages || total.back > a.pages - count) flags |= PLAN_STATE;
     else if (total.need > count + total.back) flags |= PLAN_PAGES;
-    if (total.tokens > a.max_tokens) flags |= PLAN_TOKENS;
-    const uint32_t tokens = flags ? 0u : static_cast<uint32_t>(total.tokens);
+    if (tokens_sum > a.max_tokens) flags |= PLAN_TOKENS;
+    const uint32_t tokens = flags ? 0u : static_cast<uint32_t>(tokens_sum);
     const uint32_t top = count + total.back;
     if (!flags && total.back) {
         for (uint32_t i = 0; i < NI; ++i)
@@ -201,7 +206,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PagedPlanArgs a) {
         });
     }
     __syncthreads();  // every read of lens and free_count is done: the outputs may be the inputs
-    uint32_t start = static_cast<uint32_t>(at.tokens);
+    uint32_t start = at.tokens;
 #pragma unroll
     for (uint32_t i = 0; i < NI; ++i) {
         const uint32_t r = tid * NI + i;

@@ -80,58 +80,68 @@ __device__ __forceinline__ float cache_value(uint32_t type, uint16_t bits) {
 }
 
 // A launch's share of the rows, and its scratch: parts of split tiles (BM rows of head_dim
-// sums, then their m and l), for each its tile if it is the tile's first, and their number.
+// sums, then their m and l), the split tiles, and their number.
 struct RowWork {
     uint32_t min_rows, max_rows, target, least;
     float* part;
-    uint32_t* head;   // [most_parts][4]: parts (0: not the first), request, tile, kv head
+    uint32_t* head;   // per split tile: parts, request, tile, first part's place
     uint32_t* count;  // [1]
 };
 
-// One workgroup's piece: part `part` of `parts` of row tile `tile` of request r.
+// One workgroup's piece: part `part` of `parts` of row tile `tile` of request r; its place
+// among the parts and its tile's among the split tiles, both per kv head.
 struct Piece {
-    uint32_t r, q0, fresh, tile, part, parts, slot;
+    uint32_t r, q0, fresh, tile, part, parts, slot, split;
     int32_t len;
 };
 
-// The piece of unit u, from the lengths alone: every wave finds it by itself (64 requests
-// at a time, one per lane; exclusive sums give each request its units).  total: parts of
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t dpp_from(uint32_t v) {  // 0 where there is no lane to read
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {  // inclusive sums over the lanes
+    v += dpp_from<0x111>(v);
+    v += dpp_from<0x112>(v);
+    v += dpp_from<0x114>(v);
+    v += dpp_from<0x118>(v);
+    v += dpp_from<0x142, 0xa>(v);
+    v += dpp_from<0x143, 0xc>(v);
+    return v;
+}
+
+// The piece of unit u, from the lengths alone: every wave finds it by itself, its lanes
+// taking a 64th of the requests each (exclusive sums give each request its units).  splits:
 // split tiles per kv head.
 __device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, const RowWork& w, uint32_t bm, uint32_t u,
-                                           Piece& p, uint32_t& total) {
+                                           Piece& p, uint32_t& splits) {
     const uint32_t lane = threadIdx.x & 63u, per = (a.requests + 63u) / 64u;
     const uint32_t positions = a.table_stride << a.kv.page_shift;
     auto work_of = [&](uint32_t r) -> RequestWork {
-        if (r >= a.requests) return {0u, 0u};
-        const uint32_t fresh = paged_new(a.query_start[r], a.query_start[r + 1u], a.max_new, a.max_tokens);
-        return request_work(fresh, a.lens[r], a.group, bm, w.min_rows, w.max_rows, a.window, a.sinks, positions);
+        const uint32_t at = r < a.requests ? r : 0u;
+        const uint32_t q0 = a.query_start[at], q1 = a.query_start[at + 1u], len = a.lens[at];
+        const uint32_t fresh = r < a.requests ? paged_new(q0, q1, a.max_new, a.max_tokens) : 0u;
+        return request_work(fresh, len, a.group, bm, w.min_rows, w.max_rows, a.window, a.sinks, positions);
     };
-    RequestWork one{0u, 0u};  // per == 1: the lane's request
-    uint64_t work = 0;
-    for (uint32_t i = 0; i < per; ++i) {
-        one = work_of(lane * per + i);
-        work += static_cast<uint64_t>(one.tiles) * one.keys;
+    RequestWork one = work_of(lane * per);  // where a lane has but one
+    double work = static_cast<double>(one.tiles) * one.keys;  // exact below 2^53
+    for (uint32_t i = 1; i < per; ++i) {
+        const RequestWork x = work_of(lane * per + i);
+        work += static_cast<double>(x.tiles) * x.keys;
     }
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d *= 2) work += __shfl_xor(work, d);
-    const uint64_t pieces = part_pieces(work * a.kv.kv_heads, w.target, w.least);
-    uint32_t units = 0u, slots = 0u;
+    work = lane63(group_sum<64>(work));
+    const uint64_t pieces = part_pieces(static_cast<uint64_t>(work) * a.kv.kv_heads, w.target, w.least);
+    // units, and parts and split tiles in one word (at most 2 * target, target)
+    uint32_t units = 0u, cut = 0u;
     for (uint32_t i = 0; i < per; ++i) {
         if (per > 1u) one = work_of(lane * per + i);
         const uint32_t n = request_parts(one.keys, pieces);
         units += one.tiles * n;
-        slots += n > 1u ? one.tiles * n : 0u;
+        cut += n > 1u ? one.tiles * (n + 0x10000u) : 0u;
     }
-    uint32_t eu = units, es = slots;
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d *= 2) {
-        const uint32_t x = __shfl_up(eu, d), y = __shfl_up(es, d);
-        eu += lane >= d ? x : 0u;
-        es += lane >= d ? y : 0u;
-    }
-    total = __builtin_amdgcn_readlane(es, 63);
+    uint32_t eu = wave_prefix(units), ec = wave_prefix(cut);
+    splits = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ec), 63)) >> 16;
     eu -= units;
-    es -= slots;
+    ec -= cut;
     const uint64_t mine = __ballot(u >= eu && u - eu < units);
     if (!mine) return false;
     uint32_t r = lane * per, left = u - eu;
@@ -141,16 +151,17 @@ __device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, const Ro
         r = lane * per + i;
         if (left < one.tiles * n || i + 1u == per) break;
         left -= one.tiles * n;
-        es += n > 1u ? one.tiles * n : 0u;
+        ec += n > 1u ? one.tiles * (n + 0x10000u) : 0u;
     }
     const int owner = __builtin_ctzll(mine);
     auto get = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), owner)); };
-    const uint32_t tiles = get(one.tiles), at = get(left);
+    const uint32_t tiles = get(one.tiles), at = get(left), before = get(ec);
     p.r = get(r);
     p.parts = request_parts(get(one.keys), pieces);
     p.tile = tiles - 1u - at / p.parts;  // the tiles that see most keys first
     p.part = at % p.parts;
-    p.slot = get(es) + at;
+    p.slot = (before & 0xffffu) + at;
+    p.split = (before >> 16) + at / p.parts;
     p.q0 = a.query_start[p.r];
     p.fresh = a.query_start[p.r + 1u] - p.q0;
     p.len = static_cast<int32_t>(a.lens[p.r] < positions ? a.lens[p.r] : positions);
@@ -202,14 +213,14 @@ __device__ __forceinline__ void store_row4(const PagedAttentionArgs& a, const Ro
     }
 }
 
-// The split tile's head word, written by its first part.
+// The split tile's entry, written by its first part.
 __device__ __forceinline__ void write_head(const PagedAttentionArgs& a, const RowWork& w, const Piece& p, uint32_t hk) {
-    if (p.parts == 1u) return;
-    uint32_t* h = w.head + 4u * (p.slot * a.kv.kv_heads + hk);
-    h[0] = p.part == 0u ? p.parts : 0u;
+    if (p.parts == 1u || p.part) return;
+    uint32_t* h = w.head + 4u * (p.split * a.kv.kv_heads + hk);
+    h[0] = p.parts;
     h[1] = p.r;
     h[2] = p.tile;
-    h[3] = hk;
+    h[3] = p.slot;
 }
 
 // One row over the key tiles t0 .. t1 - 1 by one wave, reading only what the row sees: for
@@ -265,6 +276,17 @@ __device__ void row_alone(const PagedAttentionArgs& a, const Piece& p, const Key
 }
 
 __device__ __forceinline__ float max_over(float v, uint32_t d) { return fmaxf(v, __shfl_xor(v, d)); }
+// The maximum with the lane 32 (16) lanes away.
+__device__ __forceinline__ float max_32(float v) {
+    const uint32_t u = __float_as_uint(v);
+    const auto w = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+}
+__device__ __forceinline__ float max_16(float v) {
+    const uint32_t u = __float_as_uint(v);
+    const auto w = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+}
 
 // A lane's part of its row: 8 values at q + at + STEP * k of each k, as parts.  F16 parts of
 // FP32 rows come under a power of two, which goes to c; the row's other lanes are MIN, 2 MIN ..
@@ -324,25 +346,29 @@ __device__ __forceinline__ void load_q(const PagedAttentionArgs& a, uint64_t at,
 // same HD / 16 columns of 8 rows and exchanges halves of its own registers, and column
 // (l % 16) * HD / 16 + e is row l % 16 of product e.  Reading K and V bounds it: the next
 // K is on its way while the weights are taken, the next V while the next scores are.
+template <uint32_t HD>
+struct RowsLds {
+    alignas(16) uint64_t off[4][32];
+    alignas(16) float o[4][16][HD + 4u];
+    float m[4][16], l[4][16];
+    uint32_t bad;
+};
+
 template <uint32_t T, uint32_t HD, bool F32>
-__global__ __launch_bounds__(256) void k_paged_rows(PagedAttentionArgs a, RowWork w) {
+__device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const RowWork& w, uint32_t block, RowsLds<HD>& lds) {
     using M = Mat<T>;
     using V8 = typename M::V8;
-    constexpr uint32_t NP = parts_of(T, F32), KK = HD / 32u, DPL = HD / 16u, BM = 16u, KT = 32u, PITCH = HD + 4u;
-    __shared__ __attribute__((aligned(16))) uint64_t s_off[4][KT];
-    __shared__ __attribute__((aligned(16))) float s_o[4][BM][PITCH];
-    __shared__ float s_m[4][BM], s_l[4][BM];
-    __shared__ uint32_t s_bad;
+    constexpr uint32_t NP = parts_of(T, F32), KK = HD / 32u, DPL = HD / 16u, BM = 16u, KT = 32u;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, g = lane >> 4, j = lane & 15u;
-    const uint32_t hk = blockIdx.x % a.kv.kv_heads;
+    const uint32_t hk = block % a.kv.kv_heads;
     Piece p;
-    uint32_t total;
-    const bool live_piece = find_piece(a, w, BM, blockIdx.x / a.kv.kv_heads, p, total);
-    if (w.count && blockIdx.x == 0u && tid == 0u) w.count[0] = total * a.kv.kv_heads;
+    uint32_t splits;
+    const bool live_piece = find_piece(a, w, BM, block / a.kv.kv_heads, p, splits);
+    if (w.count && block == 0u && tid == 0u) w.count[0] = splits * a.kv.kv_heads;
     if (!live_piece) return;
     if (tid == 0u) {
         write_head(a, w, p, hk);
-        s_bad = 0u;
+        lds.bad = 0u;
     }
     const uint32_t rows = p.fresh * a.group - p.tile * BM < BM ? p.fresh * a.group - p.tile * BM : BM;
     const uint32_t positions = a.table_stride << a.kv.page_shift, mask = (1u << a.kv.page_shift) - 1u;
@@ -376,7 +402,7 @@ __global__ __launch_bounds__(256) void k_paged_rows(PagedAttentionArgs a, RowWor
         const uint32_t i = keys.base(b, KT) + (lane & 31u);
         const bool in = page < a.kv.pages;
         there = static_cast<uint32_t>(__ballot(in));
-        s_off[wave][lane & 31u] = in ? page * a.kv.page_stride + (i & mask) * a.kv.slot_stride : 0u;
+        lds.off[wave][lane & 31u] = in ? page * a.kv.page_stride + (i & mask) * a.kv.slot_stride : 0u;
         __builtin_amdgcn_wave_barrier();
     };
     u32x4 kr[2][KK];
@@ -385,7 +411,7 @@ __global__ __launch_bounds__(256) void k_paged_rows(PagedAttentionArgs a, RowWor
     auto load_k = [&] {
 #pragma unroll
         for (uint32_t t = 0; t < 2; ++t) {
-            const uint16_t* src = kbase + s_off[wave][16u * t + j];
+            const uint16_t* src = kbase + lds.off[wave][16u * t + j];
 #pragma unroll
             for (uint32_t k = 0; k < KK; ++k) kr[t][k] = *reinterpret_cast<const u32x4*>(src + 32u * k);
         }
@@ -393,7 +419,7 @@ __global__ __launch_bounds__(256) void k_paged_rows(PagedAttentionArgs a, RowWor
     auto load_v = [&] {
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) {
-            const uint16_t* src = vbase + s_off[wave][16u * (e / 4u) + 4u * g + e % 4u];
+            const uint16_t* src = vbase + lds.off[wave][16u * (e / 4u) + 4u * g + e % 4u];
             if constexpr (VW == 2u) {
                 const u32x2 x = *reinterpret_cast<const u32x2*>(src);
                 vr[e][0] = x[0];
@@ -456,7 +482,7 @@ __global__ __launch_bounds__(256) void k_paged_rows(PagedAttentionArgs a, RowWor
         }
         float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        top = max_over(max_over(top, 16u), 32u) * c;
+        top = max_32(max_16(top)) * c;
         if (__any(top > m + kSlack)) {
             const float mm = fmaxf(m, top), keep = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mm);
             m = mm;
@@ -490,26 +516,26 @@ __global__ __launch_bounds__(256) void k_paged_rows(PagedAttentionArgs a, RowWor
     l += __shfl_xor(l, 16u);
     l += __shfl_xor(l, 32u);
     if (g == 0u) {
-        s_m[wave][j] = m;
-        s_l[wave][j] = l;
+        lds.m[wave][j] = m;
+        lds.l[wave][j] = l;
     }
     __syncthreads();
     {
-        const float mm = fmaxf(fmaxf(s_m[0][j], s_m[1][j]), fmaxf(s_m[2][j], s_m[3][j]));
+        const float mm = fmaxf(fmaxf(lds.m[0][j], lds.m[1][j]), fmaxf(lds.m[2][j], lds.m[3][j]));
         const float keep = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mm);
 #pragma unroll
         for (uint32_t x = 0; x < 4; ++x)
 #pragma unroll
             for (uint32_t e = 0; e < DPL; e += 4)
-                *reinterpret_cast<f32x4*>(&s_o[wave][j][(4u * g + x) * DPL + e]) =
+                *reinterpret_cast<f32x4*>(&lds.o[wave][j][(4u * g + x) * DPL + e]) =
                     f32x4{o[e][x] * keep, o[e + 1][x] * keep, o[e + 2][x] * keep, o[e + 3][x] * keep};
     }
     __syncthreads();
     const uint32_t row = tid / 16u;
-    const float mm = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+    const float mm = fmaxf(fmaxf(lds.m[0][row], lds.m[1][row]), fmaxf(lds.m[2][row], lds.m[3][row]));
     float sum = 0.0f;
 #pragma unroll
-    for (uint32_t v = 0; v < 4; ++v) sum += mm == -INFINITY ? s_l[v][row] : s_l[v][row] * __builtin_amdgcn_exp2f(s_m[v][row] - mm);
+    for (uint32_t v = 0; v < 4; ++v) sum += mm == -INFINITY ? lds.l[v][row] : lds.l[v][row] * __builtin_amdgcn_exp2f(lds.m[v][row] - mm);
     f32x4 r[HD / 64u];
     bool bad = false;
 #pragma unroll
@@ -517,13 +543,13 @@ __global__ __launch_bounds__(256) void k_paged_rows(PagedAttentionArgs a, RowWor
         const uint32_t d = 64u * k + 4u * (tid % 16u);
         r[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (uint32_t v = 0; v < 4; ++v) r[k] = r[k] + *reinterpret_cast<const f32x4*>(&s_o[v][row][d]);
+        for (uint32_t v = 0; v < 4; ++v) r[k] = r[k] + *reinterpret_cast<const f32x4*>(&lds.o[v][row][d]);
 #pragma unroll
         for (uint32_t x = 0; x < 4; ++x) bad = bad || r[k][x] != r[k][x];
     }
-    if (bad && row < rows) atomicOr(&s_bad, 1u << row);
+    if (bad && row < rows) atomicOr(&lds.bad, 1u << row);
     __syncthreads();
-    const uint32_t again = p_first != p_last ? s_bad : 0u;
+    const uint32_t again = p_first != p_last ? lds.bad : 0u;
     if (row < rows && !((again >> row) & 1u)) {
         const RowTo to = row_to(a, w, p, BM, hk, row);
 #pragma unroll
@@ -554,27 +580,34 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
 typedef uint8_t __attribute__((address_space(3))) * lds_ptr;
 
-// 16 bytes per lane from src into LDS, lane after lane from `to` (the same for all lanes).
-// Written out, since the builtin makes every later LDS read wait for it: the loop waits
-// itself, once per tile, before the barrier that lets the tile be read.
+// 16 bytes per lane from src (+ a lane's offset) into LDS, lane after lane from `to` (the
+// same for all lanes).  Written out, since the builtin makes every later LDS read wait for it:
+// the loop waits itself, once per tile, before the barrier that lets the tile be read.
 __device__ __forceinline__ void load_to_lds(const void* src, uint32_t to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(to) : "memory", "m0");
 }
+__device__ __forceinline__ void load_to_lds(const void* src, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(src), "s"(to)
+                 : "memory", "m0");
+}
+
+template <uint32_t HD>
+struct TilesLds {
+    alignas(1024) uint8_t k[2][kTileKeys * 2u * HD], v[2][kTileKeys * 2u * HD];
+};
 
 template <uint32_t T, uint32_t HD, bool F32>
-__global__ __launch_bounds__(256, HD <= 128u && !F32 ? 2 : 1) void k_paged_tiles(PagedAttentionArgs a, RowWork w) {
+__device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const RowWork& w, uint32_t block, TilesLds<HD>& lds) {
     using M = Mat<T>;
     using V8 = typename M::V8;
     constexpr uint32_t NP = parts_of(T, F32), KK = HD / 16u, DT = HD / 32u, BM = kTileRows, KT = kTileKeys;
     constexpr uint32_t ROWB = 2u * HD, CH = HD / 8u, RPI = 1024u / ROWB, NI = KT / RPI / 4u;
-    __shared__ __attribute__((aligned(1024))) uint8_t s_k[2][KT * ROWB], s_v[2][KT * ROWB];
-    __shared__ uint32_t s_gone[2][4];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t h = lane >> 5, j = lane & 31u, hk = blockIdx.x % a.kv.kv_heads;
+    const uint32_t h = lane >> 5, j = lane & 31u, hk = block % a.kv.kv_heads;
     Piece p;
-    uint32_t total;
-    const bool live_piece = find_piece(a, w, BM, blockIdx.x / a.kv.kv_heads, p, total);
-    if (w.count && blockIdx.x == 0u && tid == 0u) w.count[0] = total * a.kv.kv_heads;
+    uint32_t splits;
+    const bool live_piece = find_piece(a, w, BM, block / a.kv.kv_heads, p, splits);
+    if (w.count && block == 0u && tid == 0u) w.count[0] = splits * a.kv.kv_heads;
     if (!live_piece) return;
     if (tid == 0u) write_head(a, w, p, hk);
     const uint32_t left = p.fresh * a.group - p.tile * BM, rows = left < BM ? left : BM;
@@ -598,39 +631,48 @@ __global__ __launch_bounds__(256, HD <= 128u && !F32 ? 2 : 1) void k_paged_tiles
     float c = a.scale * 1.4426950408889634f;
     load_q<T, F32, KK, 16u, 32u>(a, (p.q0 + (live ? f / a.group : 0u)) * a.q_stride +
                                     (hk * a.group + (live ? f % a.group : 0u)) * HD + 8u * h, live, q, c);
-    // loads: this lane's row of each of the wave's NI pieces of a tile, 16 bytes of it
+    // Loads: the wave brings pieces wave * NI .. of RPI rows, a lane 16 bytes of one row.  Lane i
+    // asks the table for position i of the tile; where all of them are there and a piece's
+    // rows share a page, the rest is scalar: a page's address and a lane's fixed offset.
     const uint32_t* table = a.table + static_cast<uint64_t>(p.r) * a.table_stride;
     const uint32_t in_row = lane / CH;
-    const uint32_t lds_k = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)&s_k[0][0]));
-    const uint32_t lds_v = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)&s_v[0][0]));
-    uint32_t page[NI];
-    auto entries = [&](uint32_t t) {
-        const uint32_t base = keys.base(t, KT);
+    const uint32_t lds_k = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)&lds.k[0][0]));
+    const uint32_t lds_v = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)&lds.v[0][0]));
+    const bool plain = (1u << a.kv.page_shift) >= RPI && a.kv.slot_stride < (1u << 24);
+    uint32_t offset[NI];
 #pragma unroll
-        for (uint32_t n = 0; n < NI; ++n) {
-            const uint32_t i = base + (wave * NI + n) * RPI + in_row;
-            const bool in = static_cast<int32_t>(i) <= p_last && i < positions && (i >= lo || i < a.sinks);
-            page[n] = in ? table[i >> a.kv.page_shift] : kNoSlot;
-        }
+    for (uint32_t n = 0; n < NI; ++n)
+        offset[n] = 2u * (in_row * static_cast<uint32_t>(a.kv.slot_stride) +
+                          8u * ((lane % CH) ^ swizzle<HD>((wave * NI + n) * RPI + in_row)));
+    auto entry = [&](uint32_t t) -> uint32_t {
+        const uint32_t i = keys.base(t, KT) + lane;
+        const bool in = static_cast<int32_t>(i) <= p_last && i < positions && (i >= lo || i < a.sinks);
+        return in ? table[i >> a.kv.page_shift] : kNoSlot;
     };
-    auto load = [&](uint32_t t, uint32_t buf) {
+    auto load = [&](uint32_t t, uint32_t page, uint32_t buf) -> uint64_t {
         const uint32_t base = keys.base(t, KT);
-        bool gone = false;
+        const uint64_t there = __ballot(page < a.kv.pages);
+        if (plain && there == ~0ull) {
 #pragma unroll
-        for (uint32_t n = 0; n < NI; ++n) {
-            const uint32_t row = (wave * NI + n) * RPI + in_row, i = base + row;
-            const uint32_t piece = 8u * ((lane % CH) ^ swizzle<HD>(row));
-            const bool in = page[n] < a.kv.pages;
-            gone = gone || (!in && static_cast<int32_t>(i) <= p_last && (i >= lo || i < a.sinks));
-            const uint64_t off = page[n] * a.kv.page_stride + (i & mask) * a.kv.slot_stride + hk * a.kv.head_stride;
-            const uint16_t* ks = in ? a.kv.k + off : g_no_row;
-            const uint16_t* vs = in ? a.kv.v + off : g_no_row;
-            const uint32_t to = buf * KT * ROWB + (wave * NI + n) * 1024u;
-            load_to_lds(ks + piece, __builtin_amdgcn_readfirstlane(lds_k + to));
-            load_to_lds(vs + piece, __builtin_amdgcn_readfirstlane(lds_v + to));
+            for (uint32_t n = 0; n < NI; ++n) {
+                const uint32_t row = (wave * NI + n) * RPI, to = buf * KT * ROWB + (wave * NI + n) * 1024u;
+                const uint32_t pg = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(page), static_cast<int>(row)));
+                const uint64_t off = pg * a.kv.page_stride + ((base + row) & mask) * a.kv.slot_stride + hk * a.kv.head_stride;
+                load_to_lds(a.kv.k + off, offset[n], lds_k + to);
+                load_to_lds(a.kv.v + off, offset[n], lds_v + to);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t n = 0; n < NI; ++n) {
+                const uint32_t row = (wave * NI + n) * RPI + in_row, to = buf * KT * ROWB + (wave * NI + n) * 1024u;
+                const uint32_t piece = 8u * ((lane % CH) ^ swizzle<HD>(row)), pg = __shfl(page, row);
+                const uint64_t off = pg * a.kv.page_stride + ((base + row) & mask) * a.kv.slot_stride + hk * a.kv.head_stride;
+                const bool in = pg < a.kv.pages;
+                load_to_lds((in ? a.kv.k + off : g_no_row) + piece, lds_k + to);
+                load_to_lds((in ? a.kv.v + off : g_no_row) + piece, lds_v + to);
+            }
         }
-        const bool any = __any(gone);
-        if (lane == 0u) s_gone[buf][wave] = any;
+        return there;
     };
     // where this lane reads: K row j, its piece 2 k + h; V rows 4 h + 8 second + (lane % 16) / 4,
     // columns 32 dt + 16 ((lane / 16) % 2) + 4 (lane % 4)
@@ -650,18 +692,20 @@ __global__ __launch_bounds__(256, HD <= 128u && !F32 ? 2 : 1) void k_paged_tiles
 #pragma unroll
         for (uint32_t x = 0; x < 16; ++x) o[d][x] = 0.0f;
     float m = -INFINITY, l = 0.0f;
+    uint64_t next_there = 0;
+    uint32_t page = kNoSlot;
     if (t0 < t1) {
-        entries(t0);
-        load(t0, 0u);
-        if (t0 + 1u < t1) entries(t0 + 1u);
+        next_there = load(t0, entry(t0), 0u);
+        if (t0 + 1u < t1) page = entry(t0 + 1u);
     }
     for (uint32_t t = t0; t < t1; ++t) {
         const uint32_t buf = (t - t0) & 1u, base = keys.base(t, KT);
+        const uint64_t there = next_there;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of the tile have landed
         __syncthreads();                                  // and everyone's; the other buffer has been read
         if (t + 1u < t1) {
-            load(t + 1u, buf ^ 1u);
-            if (t + 2u < t1) entries(t + 2u);
+            next_there = load(t + 1u, page, buf ^ 1u);
+            if (t + 2u < t1) page = entry(t + 2u);
         }
         // nothing of the tile for this wave's rows
         if (static_cast<int32_t>(base) > w_last ||
@@ -672,7 +716,7 @@ __global__ __launch_bounds__(256, HD <= 128u && !F32 ? 2 : 1) void k_paged_tiles
         for (uint32_t ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (uint32_t x = 0; x < 16; ++x) s[ks][x] = 0.0f;
-        const uint8_t* kb = s_k[buf] + j * ROWB;
+        const uint8_t* kb = lds.k[buf] + j * ROWB;
 #pragma unroll
         for (uint32_t k = 0; k < KK; ++k)
 #pragma unroll
@@ -681,17 +725,23 @@ __global__ __launch_bounds__(256, HD <= 128u && !F32 ? 2 : 1) void k_paged_tiles
 #pragma unroll
                 for (uint32_t i = 0; i < NP; ++i) s[ks] = M::mma32(x, q[i][k], s[ks]);
             }
-        const uint32_t gone = s_gone[buf][0] | s_gone[buf][1] | s_gone[buf][2] | s_gone[buf][3];
-        if (gone || static_cast<int32_t>(base + KT) - 1 > w_first ||
+        // LDS answers late: six reads ahead of the products
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+        for (uint32_t k = 0; k < 2u * KK - 6u; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, NP, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 6u * NP, 0);
+        if (there != ~0ull || static_cast<int32_t>(base + KT) - 1 > w_first ||
             (a.window && base + a.window <= static_cast<uint32_t>(w_last) && base + KT > a.sinks)) {
+            const uint64_t mine = there >> (4u * h);
 #pragma unroll
             for (uint32_t ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (uint32_t x = 0; x < 16; ++x) {
-                    const uint32_t i = base + 32u * ks + 8u * (x / 4u) + 4u * h + x % 4u;
-                    bool seen = row_sees(pos, i, a.window, a.sinks) && i < positions;
-                    if (gone && seen) seen = table[i >> a.kv.page_shift] < a.kv.pages;
-                    if (!seen) s[ks][x] = -INFINITY;
+                    const uint32_t i = 32u * ks + 8u * (x / 4u) + x % 4u;  // + 4 h: the key in its tile
+                    if (!((mine >> i) & 1u) || !row_sees(pos, base + i + 4u * h, a.window, a.sinks)) s[ks][x] = -INFINITY;
                 }
         }
         float top = -INFINITY;
@@ -699,7 +749,7 @@ __global__ __launch_bounds__(256, HD <= 128u && !F32 ? 2 : 1) void k_paged_tiles
         for (uint32_t ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (uint32_t x = 0; x < 16; ++x) top = fmaxf(top, s[ks][x]);
-        top = max_over(top, 32u) * c;
+        top = max_32(top) * c;
         if (__any(top > m + kSlack)) {
             const float mm = fmaxf(m, top), keep = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mm);
             m = mm;
@@ -723,7 +773,7 @@ __global__ __launch_bounds__(256, HD <= 128u && !F32 ? 2 : 1) void k_paged_tiles
 #pragma unroll
                 for (uint32_t d = 0; d < DT; ++d) {
                     struct { s16x4 a, b; } x;
-                    uint8_t* vb = s_v[buf] + (32u * ks + 16u * t16) * ROWB;
+                    uint8_t* vb = lds.v[buf] + (32u * ks + 16u * t16) * ROWB;
                     x.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(vb + vat[0][d]));
                     x.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(vb + vat[1][d]));
 #pragma unroll
@@ -755,78 +805,164 @@ __global__ __launch_bounds__(256, HD <= 128u && !F32 ? 2 : 1) void k_paged_tiles
     }
 }
 
+// One launch: the tiles' workgroups first, they take longest.
+template <uint32_t T, uint32_t HD, bool F32>
+__global__ __launch_bounds__(256, HD <= 128u && !F32 ? 2 : 1) void k_paged_chunks(PagedAttentionArgs a, RowWork many,
+                                                                                RowWork few, uint32_t tile_blocks) {
+    __shared__ union Lds {
+        TilesLds<HD> tiles;
+        RowsLds<HD> rows;
+    } lds;
+    if (blockIdx.x < tile_blocks) tiles_piece<T, HD, F32>(a, many, blockIdx.x, lds.tiles);
+    else rows_piece<T, HD, F32>(a, few, blockIdx.x - tile_blocks, lds.rows);
+}
+
+template <uint32_t T, uint32_t HD, bool F32>
+__global__ __launch_bounds__(256) void k_paged_rows(PagedAttentionArgs a, RowWork few) {
+    __shared__ RowsLds<HD> lds;
+    rows_piece<T, HD, F32>(a, few, blockIdx.x, lds);
+}
+
 // ---------------------------------------------------------------------------
-// Joins the parts of split tiles.  WG (slot, y): if the slot is its tile's first part, rows
-// y * RPW .. of it: HD / 4 lanes a row, SPLIT: the rest of the workgroup over the parts, else
-// over the rows.
-template <uint32_t HD, uint32_t BM, uint32_t RPW, bool SPLIT>
-__global__ __launch_bounds__(256) void k_paged_join(PagedAttentionArgs a, RowWork w) {
-    constexpr uint32_t LANES = HD / 4u, GROUPS = 256u / LANES;
-    static_assert(!SPLIT || RPW == 1u);
-    __shared__ __attribute__((aligned(16))) float s_o[SPLIT ? GROUPS : 1u][HD];
-    __shared__ float s_m[SPLIT ? GROUPS : 1u], s_l[SPLIT ? GROUPS : 1u];
-    const uint32_t slot = blockIdx.x, tid = threadIdx.x, lane = tid % LANES, grp = tid / LANES;
-    if (slot >= w.count[0]) return;
-    const uint32_t* h = w.head + 4u * slot;
-    const uint32_t parts = h[0];
-    if (parts == 0u) return;
-    Piece p{};
-    p.r = h[1];
-    p.tile = h[2];
-    p.parts = 1u;
-    p.q0 = a.query_start[p.r];
-    p.fresh = a.query_start[p.r + 1u] - p.q0;
-    const uint32_t left = p.fresh * a.group - p.tile * BM, rows = left < BM ? left : BM;
-    const uint64_t stride = static_cast<uint64_t>(a.kv.kv_heads) * BM * (HD + 2u);
-    const float* base = w.part + static_cast<uint64_t>(slot) * BM * (HD + 2u);
-    for (uint32_t row = blockIdx.y * RPW + (SPLIT ? 0u : grp); row < blockIdx.y * RPW + RPW && row < rows;
-         row += SPLIT ? 1u : GROUPS) {
+// Joins the parts of split tiles: o = sum_i o_i 2^(m_i - m), m the parts' maximum, and l
+// likewise.  HD / 4 lanes hold a row.  Parts come from other XCDs' caches, so latency bounds
+// it: several parts' loads are on the way at once.
+constexpr uint32_t kMostParts = 2048u;
+
+struct SplitTile {
+    Piece p;
+    uint32_t parts, rows;
+    uint64_t stride;  // floats from a part to the next
+    const float* base;
+};
+__device__ __forceinline__ SplitTile split_tile(const PagedAttentionArgs& a, const RowWork& w, uint32_t bm, uint32_t i) {
+    const uint32_t* h = w.head + 4u * i;
+    const uint32_t HD = a.kv.head_dim, hk = i % a.kv.kv_heads;
+    SplitTile t{};
+    t.parts = h[0];
+    t.p.r = h[1];
+    t.p.tile = h[2];
+    t.p.parts = 1u;
+    t.p.q0 = a.query_start[t.p.r];
+    t.p.fresh = a.query_start[t.p.r + 1u] - t.p.q0;
+    const uint32_t left = t.p.fresh * a.group - t.p.tile * bm;
+    t.rows = left < bm ? left : bm;
+    t.stride = static_cast<uint64_t>(a.kv.kv_heads) * bm * (HD + 2u);
+    t.base = w.part + static_cast<uint64_t>(h[3] * a.kv.kv_heads + hk) * bm * (HD + 2u);
+    return t;
+}
+
+// 16-row tiles: few rows of up to kMostParts parts.  A workgroup takes rows y, y + step, ..,
+// its lanes share out the parts.
+template <uint32_t HD>
+__device__ __forceinline__ void join_rows(const PagedAttentionArgs& a, const RowWork& w, uint32_t i, uint32_t y, uint32_t step) {
+    constexpr uint32_t BM = 16u, LANES = HD / 4u, GROUPS = 256u / LANES, JU = 8u;
+    __shared__ __attribute__((aligned(16))) float s_o[GROUPS][HD];
+    __shared__ float s_w[kMostParts], s_red[2][4];
+    const uint32_t tid = threadIdx.x, lane = tid % LANES, grp = tid / LANES, wave = tid >> 6;
+    if (i >= w.count[0]) return;
+    const SplitTile t = split_tile(a, w, BM, i);
+    for (uint32_t row = y; row < t.rows; row += step) {
+        const float* ml = t.base + BM * HD + 2u * row;
+        float m = -INFINITY, l = 0.0f;
+        for (uint32_t k = tid; k < t.parts; k += 256u) m = fmaxf(m, ml[k * t.stride]);
+        for (uint32_t d = 1; d < 64u; d *= 2) m = max_over(m, d);
+        if ((tid & 63u) == 0u) s_red[0][wave] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+        for (uint32_t k = tid; k < t.parts; k += 256u) {
+            // m = -inf: nothing seen, or NaN alone, which has to stay
+            const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[k * t.stride] - m);
+            s_w[k] = f;
+            l += ml[k * t.stride + 1u] * f;
+        }
+        for (uint32_t d = 1; d < 64u; d *= 2) l += __shfl_xor(l, d);
+        if ((tid & 63u) == 0u) s_red[1][wave] = l;
+        __syncthreads();
+        l = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+        f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const float* at = t.base + row * HD + 4u * lane;
+        for (uint32_t k0 = grp; k0 < t.parts; k0 += GROUPS * JU) {
+            f32x4 x[JU];
+#pragma unroll
+            for (uint32_t k = 0; k < JU; ++k)
+                x[k] = *reinterpret_cast<const f32x4*>(at + (k0 + GROUPS * k < t.parts ? k0 + GROUPS * k : k0) * t.stride);
+#pragma unroll
+            for (uint32_t k = 0; k < JU; ++k)
+                if (k0 + GROUPS * k < t.parts) o = o + x[k] * s_w[k0 + GROUPS * k];
+        }
+        *reinterpret_cast<f32x4*>(&s_o[grp][4u * lane]) = o;
+        __syncthreads();
+        if (grp == 0u) {
+#pragma unroll
+            for (uint32_t k = 1; k < GROUPS; ++k) o = o + *reinterpret_cast<const f32x4*>(&s_o[k][4u * lane]);
+            store_row4(a, row_to(a, w, t.p, BM, i % a.kv.kv_heads, row), 4u * lane, o, m, l);
+        }
+        __syncthreads();
+    }
+}
+
+// 128-row tiles: many rows of few parts.  Every HD / 4 lanes take a row of their own.
+template <uint32_t HD>
+__device__ __forceinline__ void join_tiles(const PagedAttentionArgs& a, const RowWork& w, uint32_t i, uint32_t y, uint32_t step) {
+    constexpr uint32_t BM = kTileRows, LANES = HD / 4u, GROUPS = 256u / LANES, JU = 4u;
+    if (i >= w.count[0]) return;
+    const SplitTile t = split_tile(a, w, BM, i);
+    const uint32_t lane = threadIdx.x % LANES;
+    for (uint32_t row = y * GROUPS + threadIdx.x / LANES; row < t.rows; row += step * GROUPS) {
+        const float* at = t.base + row * HD + 4u * lane;
+        const float* ml = t.base + BM * HD + 2u * row;
         float m = -INFINITY, l = 0.0f;
         f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t i = SPLIT ? grp : 0u; i < parts; i += SPLIT ? GROUPS : 1u) {
-            const float* at = base + i * stride;
-            const f32x4 x = *reinterpret_cast<const f32x4*>(at + row * HD + 4u * lane);
-            const float pm = at[BM * HD + 2u * row], pl = at[BM * HD + 2u * row + 1u];
-            const float mm = fmaxf(m, pm);
-            if (mm == -INFINITY) {  // nothing seen yet, or NaN alone
-                l += pl;
-                o = o + x;
-                continue;
+        for (uint32_t k0 = 0; k0 < t.parts; k0 += JU) {
+            f32x4 x[JU];
+            float pm[JU], pl[JU], top = m;
+#pragma unroll
+            for (uint32_t k = 0; k < JU; ++k) {
+                const uint64_t to = (k0 + k < t.parts ? k0 + k : k0) * t.stride;
+                x[k] = *reinterpret_cast<const f32x4*>(at + to);
+                pm[k] = ml[to];
+                pl[k] = ml[to + 1u];
             }
-            const float k0 = __builtin_amdgcn_exp2f(m - mm), k1 = __builtin_amdgcn_exp2f(pm - mm);
-            o = o * k0 + x * k1;
-            l = l * k0 + pl * k1;
-            m = mm;
-        }
-        if constexpr (SPLIT) {
-            *reinterpret_cast<f32x4*>(&s_o[grp][4u * lane]) = o;
-            if (lane == 0u) {
-                s_m[grp] = m;
-                s_l[grp] = l;
-            }
-            __syncthreads();
-            if (grp == 0u) {
-                float mm = -INFINITY;
-                for (uint32_t i = 0; i < GROUPS; ++i) mm = fmaxf(mm, s_m[i]);
-                l = 0.0f;
-                o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                for (uint32_t i = 0; i < GROUPS; ++i) {
-                    const float k = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(s_m[i] - mm);
-                    o = o + *reinterpret_cast<const f32x4*>(&s_o[i][4u * lane]) * k;
-                    l += s_l[i] * k;
+#pragma unroll
+            for (uint32_t k = 0; k < JU; ++k) top = fmaxf(top, pm[k]);
+            const bool none = top == -INFINITY;  // nothing seen yet, or NaN alone, which has to stay
+            const float keep = none ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+            o = o * keep;
+            l *= keep;
+            m = top;
+#pragma unroll
+            for (uint32_t k = 0; k < JU; ++k)
+                if (k0 + k < t.parts) {
+                    const float f = none ? 1.0f : __builtin_amdgcn_exp2f(pm[k] - m);
+                    o = o + x[k] * f;
+                    l += pl[k] * f;
                 }
-                m = mm;
-            }
         }
-        if (!SPLIT || grp == 0u) store_row4(a, row_to(a, w, p, BM, h[3], row), 4u * lane, o, m, l);
+        store_row4(a, row_to(a, w, t.p, BM, i % a.kv.kv_heads, row), 4u * lane, o, m, l);
     }
+}
+
+template <uint32_t HD>
+__global__ __launch_bounds__(256) void k_paged_join(PagedAttentionArgs a, RowWork many, RowWork few, uint32_t many_tiles,
+                                                    uint32_t many_step, uint32_t few_tiles, uint32_t few_step) {
+    const uint32_t b = blockIdx.x, n = many_tiles * many_step;
+    if (b < n) join_tiles<HD>(a, many, b / many_step, b % many_step, many_step);
+    else join_rows<HD>(a, few, (b - n) / few_step, (b - n) % few_step, few_step);
 }
 
 // Rows of a request (new tokens times group) up to which the 16-row tiles take it.
 constexpr uint32_t kFewRows = 32u;
 // Workgroups that a launch spreads split tiles over, and a part's least work in
 // kScheduleKeys positions.
-constexpr uint32_t kRowsTarget = 1024u, kRowsLeast = 4u, kTilesTarget = 512u, kTilesLeast = 8u;
+#ifndef RT
+#define RT 1024
+#define RL 8
+#define TT 512
+#define TL 8
+#endif
+constexpr uint32_t kRowsTarget = RT, kRowsLeast = RL, kTilesTarget = TT, kTilesLeast = TL;
+static_assert(2u * kRowsTarget <= kMostParts && 2u * kTilesTarget <= kMostParts);
 
 bool may_split(const PagedAttentionArgs& a, uint32_t least) {
     const uint64_t positions = static_cast<uint64_t>(a.table_stride) << a.kv.page_shift;
@@ -839,7 +975,7 @@ struct Half {
     uint32_t bm;
     bool used, splits;
     uint64_t part_floats() const { return splits ? most_parts(w.target) * bm : 0u; }
-    uint64_t words() const { return splits ? most_parts(w.target) * 4u + 4u : 0u; }
+    uint64_t words() const { return splits ? w.target * 4u + 4u : 0u; }  // a split tile has two parts
 };
 void halves(const PagedAttentionArgs& a, Half& few, Half& many) {
     few = Half{{1u, kFewRows, kRowsTarget, kRowsLeast, nullptr, nullptr, nullptr}, 16u, a.group <= kFewRows,
@@ -854,23 +990,26 @@ template <uint32_t T, uint32_t HD, bool F32>
 hipError_t attention_t(const PagedAttentionArgs& a, const Half& few, const Half& many, hipStream_t s) {
     const uint32_t kvh = a.kv.kv_heads;
     const dim3 b(256);
-    // a call of single tokens has at most kFewRows rows of each of min(requests, tokens) requests
+    // a request of the 16-row tiles has at most kFewRows rows
     const uint64_t n = a.requests < a.max_tokens ? a.requests : a.max_tokens;
     const uint64_t few_tokens = n * (kFewRows / a.group ? kFewRows / a.group : 1u);
-    const uint64_t fu = most_units(most_tiles(few_tokens < a.max_tokens ? few_tokens : a.max_tokens, a.requests, a.group,
-                                              few.bm), kvh, few.splits ? few.w.target : 0u) * kvh;
-    const uint64_t mu = most_units(most_tiles(a.max_tokens, a.requests, a.group, many.bm), kvh,
-                                   many.splits ? many.w.target : 0u) * kvh;
+    const uint64_t ft = most_tiles(few_tokens < a.max_tokens ? few_tokens : a.max_tokens, a.requests, a.group, few.bm);
+    const uint64_t mt = most_tiles(a.max_tokens, a.requests, a.group, many.bm);
+    const uint64_t fu = most_units(ft, kvh, few.splits ? few.w.target : 0u) * kvh;
+    const uint64_t mu = most_units(mt, kvh, many.splits ? many.w.target : 0u) * kvh;
     if (fu >= (1ull << 31) || mu >= (1ull << 31)) return hipErrorInvalidValue;
+    const uint32_t tile_blocks = static_cast<uint32_t>(mu), row_blocks = few.used ? static_cast<uint32_t>(fu) : 0u;
     if (many.used)
-        hipLaunchKernelGGL((k_paged_tiles<T, HD, F32>), dim3(static_cast<uint32_t>(mu)), b, 0, s, a, many.w);
-    if (few.used)
-        hipLaunchKernelGGL((k_paged_rows<T, HD, F32>), dim3(static_cast<uint32_t>(fu)), b, 0, s, a, few.w);
-    if (many.splits)
-        hipLaunchKernelGGL((k_paged_join<HD, kTileRows, 16, false>), dim3(most_parts(many.w.target), kTileRows / 16u), b, 0,
-                           s, a, many.w);
-    if (few.splits)
-        hipLaunchKernelGGL((k_paged_join<HD, 16, 1, true>), dim3(most_parts(few.w.target), 16), b, 0, s, a, few.w);
+        hipLaunchKernelGGL((k_paged_chunks<T, HD, F32>), dim3(tile_blocks + row_blocks), b, 0, s, a, many.w, few.w, tile_blocks);
+    else
+        hipLaunchKernelGGL((k_paged_rows<T, HD, F32>), dim3(row_blocks), b, 0, s, a, few.w);
+    if (many.splits || few.splits) {
+        // split tiles, and workgroups enough for their rows: about 2048 for each kind
+        const uint32_t mn = many.splits ? static_cast<uint32_t>(mt * kvh < many.w.target ? mt * kvh : many.w.target) : 0u;
+        const uint32_t fn = few.splits ? static_cast<uint32_t>(ft * kvh < few.w.target ? ft * kvh : few.w.target) : 0u;
+        const uint32_t my = kTileRows * HD / 1024u, fy = fn <= 128u ? 16u : fn <= 1024u ? 2048u / fn : 2u;
+        hipLaunchKernelGGL(k_paged_join<HD>, dim3(mn * my + fn * fy), b, 0, s, a, many.w, few.w, mn, my, fn, fy);
+    }
     return hipGetLastError();
 }
 
@@ -901,7 +1040,7 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, float* work, hipS
         half->w.part = at;
         at += half->part_floats() * (a.kv.head_dim + 2u);
         half->w.head = reinterpret_cast<uint32_t*>(at);
-        half->w.count = half->w.head + most_parts(half->w.target) * 4u;
+        half->w.count = half->w.head + half->w.target * 4u;
         at += half->words();
     }
     const bool f32 = a.type == T_F32;
