@@ -9,6 +9,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "paged_index.hpp"
+
 namespace pk {
 
 constexpr uint32_t kNoSlot = 0xffffffffu;
@@ -60,7 +62,8 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t stream);
 struct PagedAttentionArgs {
     PagedKv kv;
     uint32_t type;            // of q and out
-    uint32_t heads, group;    // group = heads / kv_heads
+    uint32_t heads;
+    Divide group;             // heads / kv_heads
     uint32_t requests, max_tokens, max_new, table_stride;
     const void* q;
     void* out;

@@ -22,7 +22,6 @@
 
 #include "kquant.hpp"
 #include "paged.hpp"
-#include "paged_index.hpp"
 
 namespace pk {
 namespace {
@@ -82,9 +81,9 @@ __device__ __forceinline__ float cache_value(uint32_t type, uint16_t bits) {
 // A launch's share of the rows, and its scratch: parts of split tiles (BM rows of head_dim
 // sums, then their m and l), the split tiles, and their number.
 struct RowWork {
-    uint32_t min_rows, max_rows, target, least;
+    uint32_t min_rows, max_rows, log_target, least;
     float* part;
-    uint32_t* head;   // per split tile: parts, request, tile, first part's place
+    uint32_t* head;   // per split tile kHeadWords: parts, first row's q row, tokens, tile, first part's place
     uint32_t* count;  // [1]
 };
 
@@ -116,20 +115,23 @@ __device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, const Ro
                                            Piece& p, uint32_t& splits) {
     const uint32_t lane = threadIdx.x & 63u, per = (a.requests + 63u) / 64u;
     const uint32_t positions = a.table_stride << a.kv.page_shift;
+    uint32_t q0, q1, len;  // of the request asked for last
     auto work_of = [&](uint32_t r) -> RequestWork {
         const uint32_t at = r < a.requests ? r : 0u;
-        const uint32_t q0 = a.query_start[at], q1 = a.query_start[at + 1u], len = a.lens[at];
+        q0 = a.query_start[at];
+        q1 = a.query_start[at + 1u];
+        len = a.lens[at];
         const uint32_t fresh = r < a.requests ? paged_new(q0, q1, a.max_new, a.max_tokens) : 0u;
         return request_work(fresh, len, a.group, bm, w.min_rows, w.max_rows, a.window, a.sinks, positions);
     };
-    RequestWork one = work_of(lane * per);  // where a lane has but one
+    RequestWork one = work_of(lane * per);
     double work = static_cast<double>(one.tiles) * one.keys;  // exact below 2^53
     for (uint32_t i = 1; i < per; ++i) {
-        const RequestWork x = work_of(lane * per + i);
-        work += static_cast<double>(x.tiles) * x.keys;
+        one = work_of(lane * per + i);
+        work += static_cast<double>(one.tiles) * one.keys;
     }
     work = lane63(group_sum<64>(work));
-    const uint64_t pieces = part_pieces(static_cast<uint64_t>(work) * a.kv.kv_heads, w.target, w.least);
+    const uint32_t pieces = part_pieces(static_cast<uint64_t>(work) * a.kv.kv_heads, w.log_target, w.least);
     // units, and parts and split tiles in one word (at most 2 * target, target)
     uint32_t units = 0u, cut = 0u;
     for (uint32_t i = 0; i < per; ++i) {
@@ -145,8 +147,8 @@ __device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, const Ro
     const uint64_t mine = __ballot(u >= eu && u - eu < units);
     if (!mine) return false;
     uint32_t r = lane * per, left = u - eu;
-    for (uint32_t i = 0; i < per; ++i) {  // only the owner's walk matters
-        if (per > 1u) one = work_of(lane * per + i);
+    for (uint32_t i = 0; per > 1u && i < per; ++i) {  // only the owner's walk matters
+        one = work_of(lane * per + i);
         const uint32_t n = request_parts(one.keys, pieces);
         r = lane * per + i;
         if (left < one.tiles * n || i + 1u == per) break;
@@ -155,16 +157,16 @@ __device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, const Ro
     }
     const int owner = __builtin_ctzll(mine);
     auto get = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), owner)); };
-    const uint32_t tiles = get(one.tiles), at = get(left), before = get(ec);
+    const uint32_t tiles = get(one.tiles), at = get(left), before = get(ec), n = get(len);
     p.r = get(r);
     p.parts = request_parts(get(one.keys), pieces);
     p.tile = tiles - 1u - at / p.parts;  // the tiles that see most keys first
     p.part = at % p.parts;
     p.slot = (before & 0xffffu) + at;
     p.split = (before >> 16) + at / p.parts;
-    p.q0 = a.query_start[p.r];
-    p.fresh = a.query_start[p.r + 1u] - p.q0;
-    p.len = static_cast<int32_t>(a.lens[p.r] < positions ? a.lens[p.r] : positions);
+    p.q0 = get(q0);
+    p.fresh = get(q1) - p.q0;
+    p.len = static_cast<int32_t>(n < positions ? n : positions);
     return true;
 }
 
@@ -191,7 +193,7 @@ struct RowTo {
 __device__ __forceinline__ RowTo row_to(const PagedAttentionArgs& a, const RowWork& w, const Piece& p, uint32_t bm,
                                         uint32_t hk, uint32_t row) {
     const uint32_t f = p.tile * bm + row, HD = a.kv.head_dim;
-    RowTo to{a.out, (p.q0 + f / a.group) * a.out_stride + (hk * a.group + f % a.group) * HD, nullptr, nullptr};
+    RowTo to{a.out, (p.q0 + a.group(f)) * a.out_stride + (hk * a.group.by + a.group.rest(f)) * HD, nullptr, nullptr};
     if (p.parts > 1u) {
         float* base = w.part + static_cast<uint64_t>(p.slot * a.kv.kv_heads + hk) * bm * (HD + 2u);
         to.part = base + row * HD;
@@ -214,13 +216,12 @@ __device__ __forceinline__ void store_row4(const PagedAttentionArgs& a, const Ro
 }
 
 // The split tile's entry, written by its first part.
+constexpr uint32_t kHeadWords = 8u;
 __device__ __forceinline__ void write_head(const PagedAttentionArgs& a, const RowWork& w, const Piece& p, uint32_t hk) {
     if (p.parts == 1u || p.part) return;
-    uint32_t* h = w.head + 4u * (p.split * a.kv.kv_heads + hk);
-    h[0] = p.parts;
-    h[1] = p.r;
-    h[2] = p.tile;
-    h[3] = p.slot;
+    u32x4* h = reinterpret_cast<u32x4*>(w.head + kHeadWords * (p.split * a.kv.kv_heads + hk));
+    h[0] = u32x4{p.parts, p.q0, p.fresh, p.tile};
+    h[1] = u32x4{p.slot, 0u, 0u, 0u};
 }
 
 // One row over the key tiles t0 .. t1 - 1 by one wave, reading only what the row sees: for
@@ -228,9 +229,9 @@ __device__ __forceinline__ void write_head(const PagedAttentionArgs& a, const Ro
 // tile whose other rows see it.
 __device__ void row_alone(const PagedAttentionArgs& a, const Piece& p, const KeyTiles& keys, uint32_t kt, uint32_t t0,
                           uint32_t t1, uint32_t hk, uint32_t f, const RowTo& to) {
-    const uint32_t lane = threadIdx.x & 63u, HD = a.kv.head_dim, token = p.q0 + f / a.group;
-    const int32_t pos = p.len - static_cast<int32_t>(p.fresh) + static_cast<int32_t>(f / a.group);
-    const uint64_t at = token * a.q_stride + (hk * a.group + f % a.group) * HD;
+    const uint32_t lane = threadIdx.x & 63u, HD = a.kv.head_dim, token = p.q0 + a.group(f);
+    const int32_t pos = p.len - static_cast<int32_t>(p.fresh) + static_cast<int32_t>(a.group(f));
+    const uint64_t at = token * a.q_stride + (hk * a.group.by + a.group.rest(f)) * HD;
     const float c = a.scale * 1.4426950408889634f;
     const uint32_t mask = (1u << a.kv.page_shift) - 1u;
     const uint32_t* table = a.table + static_cast<uint64_t>(p.r) * a.table_stride;
@@ -370,22 +371,22 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
         write_head(a, w, p, hk);
         lds.bad = 0u;
     }
-    const uint32_t rows = p.fresh * a.group - p.tile * BM < BM ? p.fresh * a.group - p.tile * BM : BM;
+    const uint32_t rows = p.fresh * a.group.by - p.tile * BM < BM ? p.fresh * a.group.by - p.tile * BM : BM;
     const uint32_t positions = a.table_stride << a.kv.page_shift, mask = (1u << a.kv.page_shift) - 1u;
     const int32_t p0 = p.len - static_cast<int32_t>(p.fresh);
-    const int32_t p_first = p0 + static_cast<int32_t>(p.tile * BM / a.group);
-    const int32_t p_last = p0 + static_cast<int32_t>((p.tile * BM + rows - 1u) / a.group);
+    const int32_t p_first = p0 + static_cast<int32_t>(a.group(p.tile * BM));
+    const int32_t p_last = p0 + static_cast<int32_t>(a.group(p.tile * BM + rows - 1u));
     const KeyTiles keys = key_tiles(p_first, p_last, a.window, a.sinks, positions, KT);
     uint32_t b0, b1;
     part_range(keys.tiles, p.part, p.parts, b0, b1);
     // this lane's row: q parts and position
     const uint32_t f = p.tile * BM + j;
     const bool live = j < rows;
-    const int32_t pos = live ? p0 + static_cast<int32_t>(f / a.group) : -1;
+    const int32_t pos = live ? p0 + static_cast<int32_t>(a.group(f)) : -1;
     V8 q[NP][KK];
     float c = a.scale * 1.4426950408889634f;
-    load_q<T, F32, KK, 32u, 16u>(a, (p.q0 + (live ? f / a.group : 0u)) * a.q_stride +
-                                    (hk * a.group + (live ? f % a.group : 0u)) * HD + 8u * g, live, q, c);
+    load_q<T, F32, KK, 32u, 16u>(a, (p.q0 + (live ? a.group(f) : 0u)) * a.q_stride +
+                                    (hk * a.group.by + (live ? a.group.rest(f) : 0u)) * HD + 8u * g, live, q, c);
     const uint32_t* table = a.table + static_cast<uint64_t>(p.r) * a.table_stride;
     const uint16_t* kbase = a.kv.k + hk * a.kv.head_stride + 8u * g;
     const uint16_t* vbase = a.kv.v + hk * a.kv.head_stride + DPL * j;
@@ -610,11 +611,11 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
     if (w.count && block == 0u && tid == 0u) w.count[0] = splits * a.kv.kv_heads;
     if (!live_piece) return;
     if (tid == 0u) write_head(a, w, p, hk);
-    const uint32_t left = p.fresh * a.group - p.tile * BM, rows = left < BM ? left : BM;
+    const uint32_t left = p.fresh * a.group.by - p.tile * BM, rows = left < BM ? left : BM;
     const uint32_t positions = a.table_stride << a.kv.page_shift, mask = (1u << a.kv.page_shift) - 1u;
     const int32_t p0 = p.len - static_cast<int32_t>(p.fresh);
-    const int32_t p_first = p0 + static_cast<int32_t>(p.tile * BM / a.group);
-    const int32_t p_last = p0 + static_cast<int32_t>((p.tile * BM + rows - 1u) / a.group);
+    const int32_t p_first = p0 + static_cast<int32_t>(a.group(p.tile * BM));
+    const int32_t p_last = p0 + static_cast<int32_t>(a.group(p.tile * BM + rows - 1u));
     const KeyTiles keys = key_tiles(p_first, p_last, a.window, a.sinks, positions, KT);
     uint32_t t0, t1;
     part_range(keys.tiles, p.part, p.parts, t0, t1);
@@ -624,25 +625,25 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
     const uint32_t f0 = p.tile * BM + 32u * wave, f = f0 + j;
     const bool live = 32u * wave + j < rows, wave_live = 32u * wave < rows;
     const uint32_t wrows = wave_live ? (rows - 32u * wave < 32u ? rows - 32u * wave : 32u) : 0u;
-    const int32_t w_first = p0 + static_cast<int32_t>(f0 / a.group);
-    const int32_t w_last = wave_live ? p0 + static_cast<int32_t>((f0 + wrows - 1u) / a.group) : -1;
-    const int32_t pos = live ? p0 + static_cast<int32_t>(f / a.group) : -1;
+    const int32_t w_first = p0 + static_cast<int32_t>(a.group(f0));
+    const int32_t w_last = wave_live ? p0 + static_cast<int32_t>(a.group(f0 + wrows - 1u)) : -1;
+    const int32_t pos = live ? p0 + static_cast<int32_t>(a.group(f)) : -1;
     V8 q[NP][KK];
     float c = a.scale * 1.4426950408889634f;
-    load_q<T, F32, KK, 16u, 32u>(a, (p.q0 + (live ? f / a.group : 0u)) * a.q_stride +
-                                    (hk * a.group + (live ? f % a.group : 0u)) * HD + 8u * h, live, q, c);
-    // Loads: the wave brings pieces wave * NI .. of RPI rows, a lane 16 bytes of one row.  Lane i
-    // asks the table for position i of the tile; where all of them are there and a piece's
-    // rows share a page, the rest is scalar: a page's address and a lane's fixed offset.
+    load_q<T, F32, KK, 16u, 32u>(a, (p.q0 + (live ? a.group(f) : 0u)) * a.q_stride +
+                                    (hk * a.group.by + (live ? a.group.rest(f) : 0u)) * HD + 8u * h, live, q, c);
+    // Loads: the wave brings 16 rows, a lane 16 bytes of a row at a time.  Lane i asks the table
+    // for position i of the tile; where all of them are there and pages hold 16 rows or more,
+    // the rest is scalar: the address of the wave's rows and fixed offsets.
     const uint32_t* table = a.table + static_cast<uint64_t>(p.r) * a.table_stride;
     const uint32_t in_row = lane / CH;
     const uint32_t lds_k = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)&lds.k[0][0]));
     const uint32_t lds_v = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)&lds.v[0][0]));
-    const bool plain = (1u << a.kv.page_shift) >= RPI && a.kv.slot_stride < (1u << 24);
+    const bool plain = a.kv.page_shift >= 4u && a.kv.slot_stride < (1u << 26);
     uint32_t offset[NI];
 #pragma unroll
     for (uint32_t n = 0; n < NI; ++n)
-        offset[n] = 2u * (in_row * static_cast<uint32_t>(a.kv.slot_stride) +
+        offset[n] = 2u * ((n * RPI + in_row) * static_cast<uint32_t>(a.kv.slot_stride) +
                           8u * ((lane % CH) ^ swizzle<HD>((wave * NI + n) * RPI + in_row)));
     auto entry = [&](uint32_t t) -> uint32_t {
         const uint32_t i = keys.base(t, KT) + lane;
@@ -653,13 +654,13 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
         const uint32_t base = keys.base(t, KT);
         const uint64_t there = __ballot(page < a.kv.pages);
         if (plain && there == ~0ull) {
+            const uint32_t pg = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(page), static_cast<int>(16u * wave)));
+            const uint64_t off = pg * a.kv.page_stride + ((base + 16u * wave) & mask) * a.kv.slot_stride + hk * a.kv.head_stride;
+            const uint32_t to = buf * KT * ROWB + wave * NI * 1024u;
 #pragma unroll
             for (uint32_t n = 0; n < NI; ++n) {
-                const uint32_t row = (wave * NI + n) * RPI, to = buf * KT * ROWB + (wave * NI + n) * 1024u;
-                const uint32_t pg = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(page), static_cast<int>(row)));
-                const uint64_t off = pg * a.kv.page_stride + ((base + row) & mask) * a.kv.slot_stride + hk * a.kv.head_stride;
-                load_to_lds(a.kv.k + off, offset[n], lds_k + to);
-                load_to_lds(a.kv.v + off, offset[n], lds_v + to);
+                load_to_lds(a.kv.k + off, offset[n], lds_k + to + n * 1024u);
+                load_to_lds(a.kv.v + off, offset[n], lds_v + to + n * 1024u);
             }
         } else {
 #pragma unroll
@@ -835,67 +836,85 @@ struct SplitTile {
     uint64_t stride;  // floats from a part to the next
     const float* base;
 };
-__device__ __forceinline__ SplitTile split_tile(const PagedAttentionArgs& a, const RowWork& w, uint32_t bm, uint32_t i) {
-    const uint32_t* h = w.head + 4u * i;
-    const uint32_t HD = a.kv.head_dim, hk = i % a.kv.kv_heads;
-    SplitTile t{};
-    t.parts = h[0];
-    t.p.r = h[1];
-    t.p.tile = h[2];
+// Entry i, if there is one (entries past the last hold what an earlier call left).
+__device__ __forceinline__ bool split_tile(const PagedAttentionArgs& a, const RowWork& w, uint32_t bm, uint32_t i, SplitTile& t) {
+    const u32x4* h = reinterpret_cast<const u32x4*>(w.head + kHeadWords * i);
+    const uint32_t HD = a.kv.head_dim, hk = i % a.kv.kv_heads, count = w.count[0];
+    const u32x4 x = h[0];
+    const uint32_t slot = h[1][0];
+    if (i >= count) return false;
+    t.p = Piece{};
+    t.parts = x[0];
     t.p.parts = 1u;
-    t.p.q0 = a.query_start[t.p.r];
-    t.p.fresh = a.query_start[t.p.r + 1u] - t.p.q0;
-    const uint32_t left = t.p.fresh * a.group - t.p.tile * bm;
+    t.p.q0 = x[1];
+    t.p.fresh = x[2];
+    t.p.tile = x[3];
+    const uint32_t left = t.p.fresh * a.group.by - t.p.tile * bm;
     t.rows = left < bm ? left : bm;
     t.stride = static_cast<uint64_t>(a.kv.kv_heads) * bm * (HD + 2u);
-    t.base = w.part + static_cast<uint64_t>(h[3] * a.kv.kv_heads + hk) * bm * (HD + 2u);
-    return t;
+    t.base = w.part + static_cast<uint64_t>(slot * a.kv.kv_heads + hk) * bm * (HD + 2u);
+    return true;
 }
 
-// 16-row tiles: few rows of up to kMostParts parts.  A workgroup takes rows y, y + step, ..,
-// its lanes share out the parts.
+// 16-row tiles: few rows of up to kMostParts parts.  A workgroup takes rows y, y + step, ..;
+// HD / 4 lanes hold a row's sums, the others other parts, the first JU of them on the way
+// before the maxima are known.
 template <uint32_t HD>
 __device__ __forceinline__ void join_rows(const PagedAttentionArgs& a, const RowWork& w, uint32_t i, uint32_t y, uint32_t step) {
     constexpr uint32_t BM = 16u, LANES = HD / 4u, GROUPS = 256u / LANES, JU = 8u;
     __shared__ __attribute__((aligned(16))) float s_o[GROUPS][HD];
     __shared__ float s_w[kMostParts], s_red[2][4];
     const uint32_t tid = threadIdx.x, lane = tid % LANES, grp = tid / LANES, wave = tid >> 6;
-    if (i >= w.count[0]) return;
-    const SplitTile t = split_tile(a, w, BM, i);
+    SplitTile t;
+    if (!split_tile(a, w, BM, i, t)) return;
     for (uint32_t row = y; row < t.rows; row += step) {
         const float* ml = t.base + BM * HD + 2u * row;
-        float m = -INFINITY, l = 0.0f;
-        for (uint32_t k = tid; k < t.parts; k += 256u) m = fmaxf(m, ml[k * t.stride]);
-        for (uint32_t d = 1; d < 64u; d *= 2) m = max_over(m, d);
+        const float* at = t.base + row * HD + 4u * lane;
+        f32x4 x[JU];
+        auto load = [&](uint32_t k0) {
+#pragma unroll
+            for (uint32_t k = 0; k < JU; ++k) {
+                const uint32_t n = k0 + GROUPS * k;
+                x[k] = *reinterpret_cast<const f32x4*>(at + (n < t.parts ? n : 0u) * t.stride);
+            }
+        };
+        float m = tid < t.parts ? ml[tid * t.stride] : -INFINITY, l = tid < t.parts ? ml[tid * t.stride + 1u] : 0.0f;
+        const float m0 = m, l0 = l;
+        load(grp);
+        for (uint32_t k = tid + 256u; k < t.parts; k += 256u) m = fmaxf(m, ml[k * t.stride]);
+        for (uint32_t d = 1; d < 16u; d *= 2) m = max_over(m, d);
+        m = max_32(max_16(m));
         if ((tid & 63u) == 0u) s_red[0][wave] = m;
         __syncthreads();
         m = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
-        for (uint32_t k = tid; k < t.parts; k += 256u) {
-            // m = -inf: nothing seen, or NaN alone, which has to stay
-            const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[k * t.stride] - m);
+        // m = -inf: nothing seen, or NaN alone, which has to stay
+        auto weight = [&](float part_m) { return m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(part_m - m); };
+        s_w[tid] = weight(m0);
+        l = l0 * s_w[tid];
+        if (tid >= t.parts) l = 0.0f;
+        for (uint32_t k = tid + 256u; k < t.parts; k += 256u) {
+            const float f = weight(ml[k * t.stride]);
             s_w[k] = f;
             l += ml[k * t.stride + 1u] * f;
         }
-        for (uint32_t d = 1; d < 64u; d *= 2) l += __shfl_xor(l, d);
-        if ((tid & 63u) == 0u) s_red[1][wave] = l;
+        l = group_sum<64>(l);
+        if ((tid & 63u) == 63u) s_red[1][wave] = l;
         __syncthreads();
         l = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
         f32x4 o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const float* at = t.base + row * HD + 4u * lane;
-        for (uint32_t k0 = grp; k0 < t.parts; k0 += GROUPS * JU) {
-            f32x4 x[JU];
-#pragma unroll
-            for (uint32_t k = 0; k < JU; ++k)
-                x[k] = *reinterpret_cast<const f32x4*>(at + (k0 + GROUPS * k < t.parts ? k0 + GROUPS * k : k0) * t.stride);
+        for (uint32_t k0 = grp;;) {
 #pragma unroll
             for (uint32_t k = 0; k < JU; ++k)
                 if (k0 + GROUPS * k < t.parts) o = o + x[k] * s_w[k0 + GROUPS * k];
+            k0 += GROUPS * JU;
+            if (k0 >= t.parts) break;
+            load(k0);
         }
         *reinterpret_cast<f32x4*>(&s_o[grp][4u * lane]) = o;
         __syncthreads();
         if (grp == 0u) {
-#pragma unroll
-            for (uint32_t k = 1; k < GROUPS; ++k) o = o + *reinterpret_cast<const f32x4*>(&s_o[k][4u * lane]);
+            const uint32_t used = t.parts < GROUPS ? t.parts : GROUPS;
+            for (uint32_t k = 1; k < used; ++k) o = o + *reinterpret_cast<const f32x4*>(&s_o[k][4u * lane]);
             store_row4(a, row_to(a, w, t.p, BM, i % a.kv.kv_heads, row), 4u * lane, o, m, l);
         }
         __syncthreads();
@@ -906,8 +925,8 @@ __device__ __forceinline__ void join_rows(const PagedAttentionArgs& a, const Row
 template <uint32_t HD>
 __device__ __forceinline__ void join_tiles(const PagedAttentionArgs& a, const RowWork& w, uint32_t i, uint32_t y, uint32_t step) {
     constexpr uint32_t BM = kTileRows, LANES = HD / 4u, GROUPS = 256u / LANES, JU = 4u;
-    if (i >= w.count[0]) return;
-    const SplitTile t = split_tile(a, w, BM, i);
+    SplitTile t;
+    if (!split_tile(a, w, BM, i, t)) return;
     const uint32_t lane = threadIdx.x % LANES;
     for (uint32_t row = y * GROUPS + threadIdx.x / LANES; row < t.rows; row += step * GROUPS) {
         const float* at = t.base + row * HD + 4u * lane;
@@ -953,35 +972,36 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttentionArgs a, RowWor
 
 // Rows of a request (new tokens times group) up to which the 16-row tiles take it.
 constexpr uint32_t kFewRows = 32u;
-// Workgroups that a launch spreads split tiles over, and a part's least work in
-// kScheduleKeys positions.
+// Workgroups (their logarithm) that a launch spreads split tiles over, and a part's least
+// work in kScheduleKeys positions.
 #ifndef RT
-#define RT 1024
+#define RT 10
 #define RL 8
-#define TT 512
+#define TT 9
 #define TL 8
 #endif
 constexpr uint32_t kRowsTarget = RT, kRowsLeast = RL, kTilesTarget = TT, kTilesLeast = TL;
-static_assert(2u * kRowsTarget <= kMostParts && 2u * kTilesTarget <= kMostParts);
+static_assert(most_parts(1u << kRowsTarget) <= kMostParts && most_parts(1u << kTilesTarget) <= kMostParts);
 
 bool may_split(const PagedAttentionArgs& a, uint32_t least) {
     const uint64_t positions = static_cast<uint64_t>(a.table_stride) << a.kv.page_shift;
     return positions / kScheduleKeys + 2u > least + least / 4u;
 }
 
-// One of the two launches of a call, its scratch and what it needs of it.
+// The two kinds of row tiles of a call, their scratch and what they need of it.
 struct Half {
     RowWork w;
     uint32_t bm;
     bool used, splits;
-    uint64_t part_floats() const { return splits ? most_parts(w.target) * bm : 0u; }
-    uint64_t words() const { return splits ? w.target * 4u + 4u : 0u; }  // a split tile has two parts
+    uint32_t target() const { return 1u << w.log_target; }
+    uint64_t part_floats() const { return splits ? most_parts(target()) * bm : 0u; }
+    uint64_t words() const { return splits ? target() * kHeadWords + 4u : 0u; }  // a split tile has two parts
 };
 void halves(const PagedAttentionArgs& a, Half& few, Half& many) {
-    few = Half{{1u, kFewRows, kRowsTarget, kRowsLeast, nullptr, nullptr, nullptr}, 16u, a.group <= kFewRows,
+    few = Half{{1u, kFewRows, kRowsTarget, kRowsLeast, nullptr, nullptr, nullptr}, 16u, a.group.by <= kFewRows,
                may_split(a, kRowsLeast)};
     many = Half{{kFewRows + 1u, 0xffffffffu, kTilesTarget, kTilesLeast, nullptr, nullptr, nullptr}, kTileRows,
-                static_cast<uint64_t>(a.max_new) * a.group > kFewRows, may_split(a, kTilesLeast)};
+                static_cast<uint64_t>(a.max_new) * a.group.by > kFewRows, may_split(a, kTilesLeast)};
     few.splits = few.splits && few.used;
     many.splits = many.splits && many.used;
 }
@@ -992,11 +1012,11 @@ hipError_t attention_t(const PagedAttentionArgs& a, const Half& few, const Half&
     const dim3 b(256);
     // a request of the 16-row tiles has at most kFewRows rows
     const uint64_t n = a.requests < a.max_tokens ? a.requests : a.max_tokens;
-    const uint64_t few_tokens = n * (kFewRows / a.group ? kFewRows / a.group : 1u);
-    const uint64_t ft = most_tiles(few_tokens < a.max_tokens ? few_tokens : a.max_tokens, a.requests, a.group, few.bm);
-    const uint64_t mt = most_tiles(a.max_tokens, a.requests, a.group, many.bm);
-    const uint64_t fu = most_units(ft, kvh, few.splits ? few.w.target : 0u) * kvh;
-    const uint64_t mu = most_units(mt, kvh, many.splits ? many.w.target : 0u) * kvh;
+    const uint64_t few_tokens = n * (kFewRows / a.group.by ? kFewRows / a.group.by : 1u);
+    const uint64_t ft = most_tiles(few_tokens < a.max_tokens ? few_tokens : a.max_tokens, a.requests, a.group.by, few.bm);
+    const uint64_t mt = most_tiles(a.max_tokens, a.requests, a.group.by, many.bm);
+    const uint64_t fu = most_units(ft, kvh, few.splits ? few.target() : 0u) * kvh;
+    const uint64_t mu = most_units(mt, kvh, many.splits ? many.target() : 0u) * kvh;
     if (fu >= (1ull << 31) || mu >= (1ull << 31)) return hipErrorInvalidValue;
     const uint32_t tile_blocks = static_cast<uint32_t>(mu), row_blocks = few.used ? static_cast<uint32_t>(fu) : 0u;
     if (many.used)
@@ -1005,8 +1025,8 @@ hipError_t attention_t(const PagedAttentionArgs& a, const Half& few, const Half&
         hipLaunchKernelGGL((k_paged_rows<T, HD, F32>), dim3(row_blocks), b, 0, s, a, few.w);
     if (many.splits || few.splits) {
         // split tiles, and workgroups enough for their rows: about 2048 for each kind
-        const uint32_t mn = many.splits ? static_cast<uint32_t>(mt * kvh < many.w.target ? mt * kvh : many.w.target) : 0u;
-        const uint32_t fn = few.splits ? static_cast<uint32_t>(ft * kvh < few.w.target ? ft * kvh : few.w.target) : 0u;
+        const uint32_t mn = many.splits ? static_cast<uint32_t>(mt * kvh < many.target() ? mt * kvh : many.target()) : 0u;
+        const uint32_t fn = few.splits ? static_cast<uint32_t>(ft * kvh < few.target() ? ft * kvh : few.target()) : 0u;
         const uint32_t my = kTileRows * HD / 1024u, fy = fn <= 128u ? 16u : fn <= 1024u ? 2048u / fn : 2u;
         hipLaunchKernelGGL(k_paged_join<HD>, dim3(mn * my + fn * fy), b, 0, s, a, many.w, few.w, mn, my, fn, fy);
     }
@@ -1040,7 +1060,7 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, float* work, hipS
         half->w.part = at;
         at += half->part_floats() * (a.kv.head_dim + 2u);
         half->w.head = reinterpret_cast<uint32_t*>(at);
-        half->w.count = half->w.head + half->w.target * 4u;
+        half->w.count = half->w.head + half->target() * kHeadWords;
         at += half->words();
     }
     const bool f32 = a.type == T_F32;

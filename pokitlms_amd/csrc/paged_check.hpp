@@ -181,7 +181,7 @@ inline PagedCheck check_attention(const pk_hip_paged_attention* p, PagedAttentio
         if (e.error) return e;
     a.type = p->type;
     a.heads = p->heads;
-    a.group = p->heads / p->cache.kv_heads;
+    a.group = divide_by(p->heads / p->cache.kv_heads);
     a.requests = p->requests;
     a.max_tokens = p->max_tokens;
     a.max_new = p->max_new && p->max_new < p->max_tokens ? p->max_new : p->max_tokens;

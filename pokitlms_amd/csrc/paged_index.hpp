@@ -20,6 +20,21 @@ namespace pk {
 
 constexpr uint32_t kScheduleKeys = 64;  // positions of a unit of the schedule's work
 
+// n / d for n below 2^31 by a multiplication: with s = ceil(log2 d) and m = floor(2^(31 + s) /
+// d) + 1, n m / 2^(31 + s) is above n / d by less than 1 / d.
+struct Divide {
+    uint32_t by, magic, shift;
+    PK_BOTH uint32_t operator()(uint32_t n) const {
+        return static_cast<uint32_t>((static_cast<uint64_t>(n) * magic) >> shift);
+    }
+    PK_BOTH uint32_t rest(uint32_t n) const { return n - (*this)(n) * by; }
+};
+inline Divide divide_by(uint32_t d) {
+    uint32_t s = 0;
+    while ((1u << s) < d) ++s;
+    return {d, static_cast<uint32_t>((1ull << (31u + s)) / d + 1u), 31u + s};
+}
+
 // Rows of request r's new tokens for one kv head, 0 for a request that is left out.
 PK_BOTH uint32_t paged_new(uint32_t q0, uint32_t q1, uint32_t max_new, uint32_t max_tokens) {
     return q1 > q0 && q1 <= max_tokens && q1 - q0 <= max_new ? q1 - q0 : 0u;
@@ -58,26 +73,27 @@ struct RequestWork {
     uint32_t tiles;  // row tiles
     uint32_t keys;   // kScheduleKeys-sized pieces that its last row tile sees
 };
-PK_BOTH RequestWork request_work(uint32_t fresh, uint32_t len, uint32_t group, uint32_t bm, uint32_t min_rows,
+PK_BOTH RequestWork request_work(uint32_t fresh, uint32_t len, const Divide& group, uint32_t bm, uint32_t min_rows,
                                  uint32_t max_rows, uint32_t window, uint32_t sinks, uint32_t positions) {
-    const uint64_t rows = static_cast<uint64_t>(fresh) * group;
+    const uint64_t rows = static_cast<uint64_t>(fresh) * group.by;
     if (rows == 0u || rows < min_rows || rows > max_rows) return {0u, 0u};
     if (len > positions) len = positions;
     const int32_t last = static_cast<int32_t>(len) - 1;
-    const uint32_t tokens = bm / group + 1u;  // of one row tile, at most
+    const uint32_t tokens = group(bm) + 1u;  // of one row tile, at most
     const int32_t first = last - static_cast<int32_t>(tokens < fresh ? tokens : fresh) + 1;
     return {static_cast<uint32_t>((rows + bm - 1u) / bm),
             key_tiles(first < 0 ? 0 : first, last, window, sinks, positions, kScheduleKeys).tiles};
 }
 
-// Pieces per part where the launch's work (sum of tiles * keys * kv_heads) is spread over
-// `target` workgroups, at least `least`; and the parts of a request's row tiles.
-PK_BOTH uint64_t part_pieces(uint64_t work, uint32_t target, uint32_t least) {
-    const uint64_t n = (work + target - 1u) / target;
-    return n > least ? n : least;
+// Pieces per part where the launch's work (sum of tiles * keys * kv_heads, below 2^53) is
+// spread over 2^log_target workgroups, at least `least`; and the parts of a request's row
+// tiles.  A request has fewer than 2^25 pieces, so more per part need not be told apart.
+PK_BOTH uint32_t part_pieces(uint64_t work, uint32_t log_target, uint32_t least) {
+    const uint64_t n = (work + (1ull << log_target) - 1u) >> log_target;
+    return n > (1u << 28) ? 1u << 28 : n > least ? static_cast<uint32_t>(n) : least;
 }
-PK_BOTH uint32_t request_parts(uint32_t keys, uint64_t pieces) {
-    return keys <= pieces + pieces / 4u ? 1u : static_cast<uint32_t>((keys + pieces - 1u) / pieces);
+PK_BOTH uint32_t request_parts(uint32_t keys, uint32_t pieces) {
+    return keys <= pieces + pieces / 4u ? 1u : (keys + pieces - 1u) / pieces;
 }
 // Part `part` of `parts` of a tile's key tiles.
 PK_BOTH void part_range(uint32_t tiles, uint32_t part, uint32_t parts, uint32_t& t0, uint32_t& t1) {
@@ -98,6 +114,6 @@ PK_BOTH uint64_t most_units(uint64_t tiles, uint32_t kv_heads, uint32_t target) 
 }
 // Parts of split tiles, over all kv heads: a split tile sees more than 1.25 pieces, so its
 // parts are fewer than 1.8 keys / pieces.
-PK_BOTH uint64_t most_parts(uint32_t target) { return 2ull * target; }
+PK_BOTH constexpr uint64_t most_parts(uint32_t target) { return 2ull * target; }
 
 }  // namespace pk

@@ -60,7 +60,7 @@ void keys(uint32_t at) {
 
 void schedule(uint32_t at) {
     const uint32_t bm = draw(2) ? 16 : 128, group = 1 + draw(draw(2) ? 9 : 70), kv_heads = 1 + draw(8);
-    const uint32_t target = 1u << draw(11), least = 1 + draw(8), requests = 1 + draw(40);
+    const uint32_t log_target = draw(11), target = 1u << log_target, least = 1 + draw(8), requests = 1 + draw(40);
     const uint32_t min_rows = draw(2) ? 1 : 33, max_rows = draw(2) ? 32 : 0xffffffffu;
     const uint32_t window = draw(3) ? 0 : 1 + draw(3000), sinks = draw(200), positions = 64 + draw(40000);
     const uint32_t tokens = 1 + draw(3000), max_new = 1 + draw(tokens);
@@ -76,12 +76,13 @@ void schedule(uint32_t at) {
     for (uint32_t r = 0; r < requests; ++r) {
         const uint32_t fresh = pk::paged_new(start[r], start[r + 1], max_new, tokens);
         CHECK(fresh == (start[r + 1] - start[r] > max_new ? 0 : start[r + 1] - start[r]));
-        all.push_back(pk::request_work(fresh, lens[r], group, bm, min_rows, max_rows, window, sinks, positions));
+        all.push_back(pk::request_work(fresh, lens[r], pk::divide_by(group), bm, min_rows, max_rows, window, sinks, positions));
         const uint64_t rows = uint64_t(fresh) * group;
         CHECK(all[r].tiles == (rows >= min_rows && rows <= max_rows ? (rows + bm - 1) / bm : 0));
         work += uint64_t(all[r].tiles) * all[r].keys;
     }
-    const uint64_t pieces = pk::part_pieces(work * kv_heads, target, least);
+    const uint32_t pieces = pk::part_pieces(work * kv_heads, log_target, least);
+    CHECK(pieces >= least && uint64_t(pieces) * target >= work * kv_heads);
     uint64_t units = 0, parts = 0;
     for (const pk::RequestWork& r : all) {
         const uint32_t n = pk::request_parts(r.keys, pieces);
@@ -93,6 +94,14 @@ void schedule(uint32_t at) {
     CHECK(parts * kv_heads <= pk::most_parts(target));
     // a cache whose rows are too short to be split has no parts
     if (positions / pk::kScheduleKeys + 2 <= least + least / 4) CHECK(parts == 0);
+}
+
+void divide(uint32_t at) {
+    const uint32_t d = 1 + draw(at % 2 ? 40 : 5000);
+    const pk::Divide by = pk::divide_by(d);
+    for (const uint32_t n : {0u, 1u, d - 1, d, d + 1, draw(0x7fffffff), 0x7fffffffu, 0x7fffffffu / d * d,
+                             0x7fffffffu / d * d - 1, draw(100000)})
+        CHECK(by(n) == n / d && by.rest(n) == n % d);
 }
 
 void bad_lengths(uint32_t at) {
@@ -108,6 +117,7 @@ int main() {
     for (; at < 3000; ++at) keys(at);
     for (; at < 60000; ++at) schedule(at);
     for (; at < 80000; ++at) bad_lengths(at);
+    for (; at < 100000; ++at) divide(at);
     std::printf("ok %u\n", at);
     return 0;
 }
