@@ -2236,7 +2236,7 @@ pk_hip_status pk_hip_paged_attention_async(pk_hip_ctx* ctx, const pk_hip_paged_a
                           if (floats) ctx->attn_work.ensure(floats);
                           launch_checked(pk::launch_paged_attention(a, ctx->attn_work.ptr, s),
                                          "paged attention launch");
-                          ++ctx->stats.dispatches;
+                          ctx->stats.dispatches += pk::paged_attention_launches(a);
                       });
     });
 }

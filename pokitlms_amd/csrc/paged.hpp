@@ -74,6 +74,7 @@ struct PagedAttentionArgs {
 };
 // work: paged_attention_work_floats(a) floats of scratch, 16-byte aligned.
 size_t paged_attention_work_floats(const PagedAttentionArgs& a);
+uint32_t paged_attention_launches(const PagedAttentionArgs& a);
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, float* work, hipStream_t stream);
 
 }  // namespace pk

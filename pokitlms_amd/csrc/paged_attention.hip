@@ -972,64 +972,63 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttentionArgs a, RowWor
 
 // Rows of a request (new tokens times group) up to which the 16-row tiles take it.
 constexpr uint32_t kFewRows = 32u;
-// Workgroups (their logarithm) that a launch spreads split tiles over, and a part's least
-// work in kScheduleKeys positions.
-#ifndef RT
-#define RT 10
-#define RL 8
-#define TT 9
-#define TL 8
-#endif
-constexpr uint32_t kRowsTarget = RT, kRowsLeast = RL, kTilesTarget = TT, kTilesLeast = TL;
-static_assert(most_parts(1u << kRowsTarget) <= kMostParts && most_parts(1u << kTilesTarget) <= kMostParts);
 
-bool may_split(const PagedAttentionArgs& a, uint32_t least) {
-    const uint64_t positions = static_cast<uint64_t>(a.table_stride) << a.kv.page_shift;
-    return positions / kScheduleKeys + 2u > least + least / 4u;
-}
+// How far long rows are cut: workgroups that split tiles are spread over (the logarithm) and
+// a part's least work in kScheduleKeys positions.  Measured with 32 heads over 4 of 128:
+// 64 requests of up to 8192 positions in 1024 parts of 16-row tiles 78.5 us, in 512 81.7
+// (512 workgroups are resident, but requests are uneven); one request of 131,072 in 1024
+// 61.7 us, in 512 57.7 (all alike, and half the parts to join), so calls of few tiles take
+// 512.  128-row tiles (24 requests, six chunks of 512): 512 parts 120 us, 256 132, 1024 141.
+// Least work of 8 pieces: eight requests of 512 in one part each 10.9 us, in two (least 4)
+// 13.9; 16 chunks under a window of 1024 in two or three parts 40 us, whole (least 16) 59.
+constexpr uint32_t kRowsTarget = 10u, kFewTilesTarget = 9u, kTilesTarget = 9u, kLeast = 8u;
+constexpr uint64_t kFewTiles = 64u;
+static_assert(most_parts(1u << kRowsTarget) <= kMostParts && most_parts(1u << kTilesTarget) <= kMostParts);
 
 // The two kinds of row tiles of a call, their scratch and what they need of it.
 struct Half {
     RowWork w;
     uint32_t bm;
     bool used, splits;
+    uint64_t tiles;  // at most, over all kv heads
     uint32_t target() const { return 1u << w.log_target; }
     uint64_t part_floats() const { return splits ? most_parts(target()) * bm : 0u; }
     uint64_t words() const { return splits ? target() * kHeadWords + 4u : 0u; }  // a split tile has two parts
+    uint64_t units(uint32_t kv_heads) const { return most_units(tiles / kv_heads, kv_heads, splits ? target() : 0u) * kv_heads; }
+    uint32_t split_tiles() const { return !splits ? 0u : tiles < target() ? static_cast<uint32_t>(tiles) : target(); }
 };
 void halves(const PagedAttentionArgs& a, Half& few, Half& many) {
-    few = Half{{1u, kFewRows, kRowsTarget, kRowsLeast, nullptr, nullptr, nullptr}, 16u, a.group.by <= kFewRows,
-               may_split(a, kRowsLeast)};
-    many = Half{{kFewRows + 1u, 0xffffffffu, kTilesTarget, kTilesLeast, nullptr, nullptr, nullptr}, kTileRows,
-                static_cast<uint64_t>(a.max_new) * a.group.by > kFewRows, may_split(a, kTilesLeast)};
-    few.splits = few.splits && few.used;
-    many.splits = many.splits && many.used;
+    const uint64_t positions = static_cast<uint64_t>(a.table_stride) << a.kv.page_shift;
+    const bool may_split = positions / kScheduleKeys + 2u > kLeast + kLeast / 4u;
+    const uint32_t group = a.group.by;
+    // a request of the 16-row tiles has at most kFewRows rows
+    const uint64_t n = a.requests < a.max_tokens ? a.requests : a.max_tokens;
+    const uint64_t tokens = n * (kFewRows / group ? kFewRows / group : 1u);
+    few = Half{{1u, kFewRows, kRowsTarget, kLeast, nullptr, nullptr, nullptr}, 16u, group <= kFewRows, false,
+               most_tiles(tokens < a.max_tokens ? tokens : a.max_tokens, a.requests, group, 16u) * a.kv.kv_heads};
+    if (few.tiles < kFewTiles) few.w.log_target = kFewTilesTarget;
+    many = Half{{kFewRows + 1u, 0xffffffffu, kTilesTarget, kLeast, nullptr, nullptr, nullptr}, kTileRows,
+                static_cast<uint64_t>(a.max_new) * group > kFewRows, false,
+                most_tiles(a.max_tokens, a.requests, group, kTileRows) * a.kv.kv_heads};
+    few.splits = may_split && few.used;
+    many.splits = may_split && many.used;
 }
 
 template <uint32_t T, uint32_t HD, bool F32>
 hipError_t attention_t(const PagedAttentionArgs& a, const Half& few, const Half& many, hipStream_t s) {
-    const uint32_t kvh = a.kv.kv_heads;
-    const dim3 b(256);
-    // a request of the 16-row tiles has at most kFewRows rows
-    const uint64_t n = a.requests < a.max_tokens ? a.requests : a.max_tokens;
-    const uint64_t few_tokens = n * (kFewRows / a.group.by ? kFewRows / a.group.by : 1u);
-    const uint64_t ft = most_tiles(few_tokens < a.max_tokens ? few_tokens : a.max_tokens, a.requests, a.group.by, few.bm);
-    const uint64_t mt = most_tiles(a.max_tokens, a.requests, a.group.by, many.bm);
-    const uint64_t fu = most_units(ft, kvh, few.splits ? few.target() : 0u) * kvh;
-    const uint64_t mu = most_units(mt, kvh, many.splits ? many.target() : 0u) * kvh;
-    if (fu >= (1ull << 31) || mu >= (1ull << 31)) return hipErrorInvalidValue;
-    const uint32_t tile_blocks = static_cast<uint32_t>(mu), row_blocks = few.used ? static_cast<uint32_t>(fu) : 0u;
+    const uint64_t fu = few.used ? few.units(a.kv.kv_heads) : 0u, mu = many.used ? many.units(a.kv.kv_heads) : 0u;
+    if (fu + mu >= (1ull << 31)) return hipErrorInvalidValue;
+    const dim3 g(static_cast<uint32_t>(fu + mu)), b(256);
     if (many.used)
-        hipLaunchKernelGGL((k_paged_chunks<T, HD, F32>), dim3(tile_blocks + row_blocks), b, 0, s, a, many.w, few.w, tile_blocks);
+        hipLaunchKernelGGL((k_paged_chunks<T, HD, F32>), g, b, 0, s, a, many.w, few.w, static_cast<uint32_t>(mu));
     else
-        hipLaunchKernelGGL((k_paged_rows<T, HD, F32>), dim3(row_blocks), b, 0, s, a, few.w);
-    if (many.splits || few.splits) {
-        // split tiles, and workgroups enough for their rows: about 2048 for each kind
-        const uint32_t mn = many.splits ? static_cast<uint32_t>(mt * kvh < many.target() ? mt * kvh : many.target()) : 0u;
-        const uint32_t fn = few.splits ? static_cast<uint32_t>(ft * kvh < few.target() ? ft * kvh : few.target()) : 0u;
-        const uint32_t my = kTileRows * HD / 1024u, fy = fn <= 128u ? 16u : fn <= 1024u ? 2048u / fn : 2u;
-        hipLaunchKernelGGL(k_paged_join<HD>, dim3(mn * my + fn * fy), b, 0, s, a, many.w, few.w, mn, my, fn, fy);
-    }
+        hipLaunchKernelGGL((k_paged_rows<T, HD, F32>), g, b, 0, s, a, few.w);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess || !(many.splits || few.splits)) return err;
+    // workgroups enough for the split tiles' rows: about 2048 of each kind
+    const uint32_t mn = many.split_tiles(), fn = few.split_tiles();
+    const uint32_t my = kTileRows * HD / 1024u, fy = fn <= 128u ? 16u : 2048u / fn;
+    hipLaunchKernelGGL(k_paged_join<HD>, dim3(mn * my + fn * fy), b, 0, s, a, many.w, few.w, mn, my, fn, fy);
     return hipGetLastError();
 }
 
@@ -1044,6 +1043,12 @@ hipError_t attention_hd(const PagedAttentionArgs& a, const Half& few, const Half
 }
 
 }  // namespace
+
+uint32_t paged_attention_launches(const PagedAttentionArgs& a) {
+    Half few, many;
+    halves(a, few, many);
+    return few.splits || many.splits ? 2u : 1u;
+}
 
 size_t paged_attention_work_floats(const PagedAttentionArgs& a) {
     Half few, many;
