@@ -394,6 +394,28 @@ pk_hip_status pk_hip_qwen3moe_generate(pk_hip_qwen3moe* model, const uint32_t* p
                                        float* last_logits, pk_hip_generation_stats* stats,
                                        char* error_buffer, size_t error_capacity);
 
+/* One request of pk_hip_qwen3moe_generate_batch; host memory. */
+typedef struct pk_hip_batch_request {
+    const uint32_t* prompt;
+    uint32_t n_prompt, n_new;
+    uint32_t* out_tokens;  /* [n_new] */
+    float* last_logits;    /* [vocab], the logits after the last prompt token; or NULL */
+} pk_hip_batch_request;
+
+/* pk_hip_qwen3moe_generate for many requests at once over one paged KV cache (no
+ * counterpart in the reference, whose runner holds one sequence): every step takes a row
+ * of each request that decodes and fills up to 512 rows with rows of prompts, all of them
+ * through the projections, the experts and the attention together; a request that is done
+ * gives its pages to the next.  Each request's tokens and logits are those of its own
+ * pk_hip_qwen3moe_generate within FP32 reassociation (fast mode; the same window of
+ * kv_capacity positions).  Reference-order models and those whose prompts are not batched
+ * return UNSUPPORTED.  Memory for the pages is taken for the call; where it is short, fewer
+ * requests are on their way at once.  stats: prefill_ns wall time until the last prompt
+ * is through, decode_ns wall time of the steps after it, sums of tokens and forwards. */
+pk_hip_status pk_hip_qwen3moe_generate_batch(pk_hip_qwen3moe* model, const pk_hip_batch_request* requests,
+                                             uint32_t n_requests, pk_hip_generation_stats* stats,
+                                             char* error_buffer, size_t error_capacity);
+
 /* Seeded synthetic weights made in HBM (no counterpart in the reference: the
  * benchmark and test models, byte-identical to pokitlms_amd/synth_model.py):
  * word i = splitmix64(key + i), then the scale fix-up `kind` (0 none, 1

@@ -35,7 +35,7 @@ EXPORTS = (
     "pk_hip_expf_block_sums", "pk_hip_rmsnorm", "pk_hip_add_rmsnorm", "pk_hip_matvec_add_rmsnorm", "pk_hip_attention_steps",
     "pk_hip_read_floor_async", "pk_hip_moe_decode_traced_async", "pk_hip_set_libm_expf",
     "pk_hip_moe_decode_reference_order", "pk_hip_paged_plan_async", "pk_hip_paged_append_async",
-    "pk_hip_paged_attention_async",
+    "pk_hip_paged_attention_async", "pk_hip_qwen3moe_generate_batch",
 )
 TRACE_WORDS = 3 * 8192 * 8
 
@@ -132,6 +132,12 @@ class PagedAttentionDesc(ctypes.Structure):
         ("scale", ctypes.c_float), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p),
         ("q_stride", ctypes.c_uint64), ("out_stride", ctypes.c_uint64)] + [
         (n, ctypes.c_void_p) for n in ("query_start", "lens", "block_table")]
+
+
+class BatchRequest(ctypes.Structure):
+    _fields_ = [("prompt", ctypes.c_void_p), ("n_prompt", ctypes.c_uint32),
+                ("n_new", ctypes.c_uint32), ("out_tokens", ctypes.c_void_p),
+                ("last_logits", ctypes.c_void_p)]
 
 
 class GenerationStats(ctypes.Structure):
@@ -250,6 +256,9 @@ def lib() -> ctypes.CDLL:
                                            ctypes.POINTER(GenerationStats), cp, sz]
     L.pk_hip_synth_weight.restype = ctypes.c_int
     L.pk_hip_synth_weight.argtypes = [vp, u32, u64, u64, u32, u64, u32, ctypes.POINTER(vp), cp, sz]
+    L.pk_hip_qwen3moe_generate_batch.restype = ctypes.c_int
+    L.pk_hip_qwen3moe_generate_batch.argtypes = [vp, ctypes.POINTER(BatchRequest), u32,
+                                                 ctypes.POINTER(GenerationStats), cp, sz]
     for name, desc in (("pk_hip_paged_plan_async", PagedPlanDesc),
                        ("pk_hip_paged_append_async", PagedAppendDesc),
                        ("pk_hip_paged_attention_async", PagedAttentionDesc)):

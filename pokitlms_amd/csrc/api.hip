@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "../../include/pokit_hip.h"
+#include "batch_schedule.hpp"
 #include "chunk_scratch.hpp"
 #include "launch.hpp"
 #include "layout.hpp"
@@ -1855,6 +1856,218 @@ pk_hip_status pk_hip_qwen3moe_generate(pk_hip_qwen3moe* m, const uint32_t* promp
     });
 }
 
+pk_hip_status pk_hip_qwen3moe_generate_batch(pk_hip_qwen3moe* m, const pk_hip_batch_request* requests,
+                                             uint32_t n_requests, pk_hip_generation_stats* stats, char* err,
+                                             size_t cap) {
+    pk_hip_ctx* ctx = m ? m->ctx : nullptr;
+    return guarded(ctx, err, cap, [&] {
+        require_usable(ctx);
+        if (!requests || n_requests == 0) throw ArgError("at least one request is required");
+        const pk::ModelArgs& a = m->args;
+        std::vector<uint32_t> n_prompt(n_requests), n_new(n_requests), start(n_requests);
+        uint64_t words = 0, prompt_tokens = 0, forwards = 0;
+        for (uint32_t r = 0; r < n_requests; ++r) {
+            const pk_hip_batch_request& q = requests[r];
+            if (!q.prompt || q.n_prompt == 0 || (q.n_new && !q.out_tokens))
+                throw ArgError("every request needs a prompt and an output buffer");
+            for (uint32_t i = 0; i < q.n_prompt; ++i)
+                if (q.prompt[i] >= a.vocab) throw ArgError("token id exceeds model vocabulary");
+            if (uint64_t(q.n_prompt) + q.n_new > m->cfg.context)
+                throw ArgError("prompt and new tokens exceed the model context");
+            n_prompt[r] = q.n_prompt;
+            n_new[r] = q.n_new;
+            start[r] = static_cast<uint32_t>(words);
+            words += uint64_t(q.n_prompt) + q.n_new + 1;
+            if (words >= (1ull << 31)) throw ArgError("too many tokens in one batch");
+            prompt_tokens += q.n_prompt;
+            forwards += pk::batch_positions(q.n_prompt, q.n_new) - q.n_prompt;
+        }
+        if (!pk::prompt_supported(a, m->layers.data()))
+            throw Unsupported("batched generation covers fast-mode models whose prompts are batched");
+        std::lock_guard lock(ctx->mutex);
+        ctx->set_device();
+        hipStream_t s = ctx->stream;
+        pk::PromptArgs pa{};
+        if (!prompt_scratch_ready(m, static_cast<uint32_t>(std::min<uint64_t>(prompt_tokens, pk::kPromptTokens)), pa))
+            throw std::runtime_error("not enough device memory for a batch");
+        const uint32_t budget = m->prompt.tokens, qd = a.heads * a.head_dim, kd = a.kv_heads * a.head_dim;
+        uint32_t head_batch = 1;
+        while (head_batch < 8 && pk::matvec_supported(a.out_type, a.hidden, head_batch + 1)) ++head_batch;
+        size_t head_floats = 0;
+        for (uint32_t k = 1; k <= head_batch; ++k)
+            head_floats = std::max(head_floats, pk::matvec_partial_floats(a.out_type, a.hidden, k, a.vocab));
+        // the batch's memory, given back at the end; with fewer requests at once where it is short
+        constexpr uint32_t kPage = 16, kMostSlots = 256;
+        struct Block {
+            uint8_t* mem = nullptr;
+            ~Block() { if (mem) (void)hipFree(mem); }
+        } block;
+        pk::BatchSchedule plan;
+        pk::BatchArgs b{};
+        uint32_t *lens = nullptr, *count = nullptr, *schedule = nullptr, *starts = nullptr;
+        for (uint32_t slots = std::min({n_requests, budget, kMostSlots});; slots /= 2) {
+            if (slots == 0) throw std::runtime_error("not enough device memory for a batch");
+            plan = pk::batch_schedule(n_prompt, n_new, slots, budget, kPage);
+            b = pk::BatchArgs{};
+            pk::PagedPlanArgs& p = b.plan;
+            p.requests = slots;
+            p.page_shift = pk::paged_shift(kPage);
+            p.pages = plan.pages;
+            p.table_stride = plan.width;
+            pk::PagedAttentionArgs& t = b.attention;
+            t.kv = pk::PagedKv{nullptr, nullptr, 1u, plan.pages, p.page_shift, a.kv_heads, a.head_dim,
+                               uint64_t(kd) * kPage, kd, a.head_dim};
+            t.heads = a.heads;
+            t.group = pk::divide_by(a.heads / a.kv_heads);
+            t.requests = slots;
+            t.table_stride = plan.width;
+            t.q_stride = t.out_stride = qd;
+            t.scale = a.attn_scale;
+            t.window = a.capacity;  // as the ring: the last kv_capacity positions
+            size_t attention_floats = 0;
+            for (const pk::BatchStep& step : plan.steps) {
+                t.max_tokens = step.rows;
+                t.max_new = step.most_new;
+                attention_floats = std::max(attention_floats, pk::paged_attention_work_floats(t));
+            }
+            b.layer_kv = uint64_t(plan.pages) * kPage * kd;
+            uint64_t at = 0;
+            auto layout = [&](uint8_t* base) {
+                at = 0;
+                auto take = [&](auto*& q, uint64_t n) {
+                    using P = std::remove_reference_t<decltype(*q)>;
+                    q = reinterpret_cast<P*>(base + at);
+                    at += (n * sizeof(P) + 255) / 256 * 256;
+                };
+                take(schedule, plan.words.size());
+                take(starts, n_requests);
+                take(lens, slots);
+                take(count, 4);
+                take(p.table, uint64_t(slots) * plan.width);
+                take(p.free_pages, plan.pages);
+                take(p.query_start, slots + 1);
+                take(p.positions, budget);
+                take(p.slots, budget);
+                take(p.token_request, budget);
+                take(b.row_tokens, budget);
+                take(p.status, 4);
+                take(b.flags, 4);
+                take(b.zero, 4);
+                take(b.tokens, words);
+                take(b.att, uint64_t(budget) * qd);
+                take(b.normed, uint64_t(plan.most_selected) * a.hidden);
+                take(b.logits, uint64_t(plan.most_selected) * a.vocab);
+                take(b.head_work, head_floats);
+                take(b.attention_work, attention_floats);
+                take(b.kv, 2ull * a.layers * b.layer_kv);
+            };
+            layout(nullptr);
+            block.mem = prompt_alloc(at);
+            if (!block.mem) continue;
+            layout(block.mem);
+            break;
+        }
+        pk::PagedPlanArgs& p = b.plan;
+        p.lens = p.lens_out = lens;
+        p.free_count = p.free_count_out = count;
+        b.attention.query_start = p.query_start;
+        b.attention.lens = lens;
+        b.attention.table = p.table;
+        b.head_batch = head_batch;
+        b.token_start = starts;
+        pk::PagedAppendArgs& ap = b.append;
+        ap.kv = b.attention.kv;
+        ap.heads = a.heads;
+        ap.rotary_pairs = a.head_dim / 2;
+        ap.axes = 1;
+        ap.eps = a.rms_eps;
+        ap.q_out_stride = qd;
+        ap.positions = p.positions;
+        ap.slots = p.slots;
+        pk::rotary_turns(ap, a.rope_theta);
+        std::vector<uint32_t> tokens(words, 0), pages(plan.pages);
+        for (uint32_t r = 0; r < n_requests; ++r)
+            std::copy(requests[r].prompt, requests[r].prompt + n_prompt[r], tokens.begin() + start[r]);
+        for (uint32_t i = 0; i < plan.pages; ++i) pages[i] = plan.pages - 1 - i;
+        const std::vector<uint32_t> zeros(std::max<size_t>(p.requests, 4), 0);
+        auto up = [&](uint32_t* to, const uint32_t* from, size_t n) {
+            check(hipMemcpyAsync(to, from, n * sizeof(uint32_t), hipMemcpyHostToDevice, s), "copy batch");
+        };
+        up(schedule, plan.words.data(), plan.words.size());
+        up(starts, start.data(), n_requests);
+        up(lens, zeros.data(), p.requests);
+        up(count, &plan.pages, 1);
+        up(p.free_pages, pages.data(), pages.size());
+        up(b.flags, zeros.data(), 4);
+        up(b.zero, zeros.data(), 4);
+        up(b.tokens, tokens.data(), words);
+        check(hipStreamSynchronize(s), "hipStreamSynchronize");
+        const auto t0 = std::chrono::steady_clock::now();
+        auto t1 = t0;
+        uint64_t prompt_left = prompt_tokens;
+        std::vector<uint64_t> done(n_requests, 0);
+        for (const pk::BatchStep& step : plan.steps) {
+            const uint32_t* hw = plan.words.data() + step.at;
+            const uint32_t* dw = schedule + step.at;
+            p.new_lens = dw;
+            p.release = dw + p.requests;
+            b.slot_request = dw + 2 * p.requests;
+            b.select = dw + 3 * p.requests;
+            b.rows = b.append.tokens = p.max_tokens = b.attention.max_tokens = step.rows;
+            b.append.position_stride = step.rows;
+            b.attention.max_new = step.most_new;
+            b.selected = step.selected;
+            check(pk::launch_batch_step(pa, m->layers.data(), b, s), "batch step");
+            bool prompts = false;
+            for (uint32_t i = 0; i < p.requests; ++i) {
+                const uint32_t r = hw[2 * p.requests + i];
+                if (!hw[i]) continue;
+                if (done[r] < n_prompt[r]) {
+                    prompts = true;
+                    prompt_left -= hw[i];
+                }
+                done[r] += hw[i];
+            }
+            for (uint32_t i = 0; i < step.selected; ++i) {
+                const uint32_t r = hw[3 * p.requests + 2 * i + 1];
+                if (requests[r].last_logits && done[r] == n_prompt[r])
+                    check(hipMemcpyAsync(requests[r].last_logits, b.logits + uint64_t(i) * a.vocab,
+                                         uint64_t(a.vocab) * sizeof(float), hipMemcpyDeviceToHost, s),
+                          "copy logits");
+            }
+            if (prompts && prompt_left == 0) {
+                check(hipStreamSynchronize(s), "hipStreamSynchronize");
+                t1 = std::chrono::steady_clock::now();
+            }
+        }
+        uint32_t flags[4] = {}, moe_flags[4] = {};
+        check(hipMemcpyAsync(flags, b.flags, sizeof(flags), hipMemcpyDeviceToHost, s), "read state");
+        check(hipMemcpyAsync(moe_flags, m->moe_status.ptr, sizeof(moe_flags), hipMemcpyDeviceToHost, s),
+              "read router status");
+        check(hipMemcpyAsync(tokens.data(), b.tokens, words * sizeof(uint32_t), hipMemcpyDeviceToHost, s), "copy tokens");
+        check(hipStreamSynchronize(s), "hipStreamSynchronize");
+        const auto t2 = std::chrono::steady_clock::now();
+        if (moe_flags[0] || flags[0] || flags[1]) {
+            const uint32_t zero[4] = {};
+            (void)hipMemcpy(m->moe_status.ptr, zero, sizeof(zero), hipMemcpyHostToDevice);
+            throw std::runtime_error(flags[1]      ? "a batch step did not fit its pages"
+                                     : moe_flags[0] ? "expert router produced non-finite logits"
+                                                    : "model produced non-finite logits");
+        }
+        for (uint32_t r = 0; r < n_requests; ++r)
+            std::copy_n(tokens.begin() + start[r] + n_prompt[r], n_new[r], requests[r].out_tokens);
+        if (stats) {
+            auto ns = [](auto d) {
+                return static_cast<uint64_t>(std::chrono::duration_cast<std::chrono::nanoseconds>(d).count());
+            };
+            stats->prefill_ns = ns(t1 - t0);
+            stats->decode_ns = ns(t2 - t1);
+            stats->prompt_tokens = static_cast<uint32_t>(prompt_tokens);
+            stats->decode_forwards = static_cast<uint32_t>(forwards);
+        }
+    });
+}
+
 pk_hip_status pk_hip_synth_weight(pk_hip_ctx* ctx, uint32_t type, uint64_t in, uint64_t out,
                                   uint32_t n_experts, uint64_t key, uint32_t kind,
                                   pk_hip_weight** out_w, char* err, size_t cap) {
@@ -2213,9 +2426,7 @@ pk_hip_status pk_hip_paged_append_async(pk_hip_ctx* ctx, const pk_hip_paged_appe
         require(pk::check_append(append, a));
         require_usable(ctx);
         std::lock_guard lock(ctx->mutex);
-        for (uint32_t i = 0; i < a.rotary_pairs; ++i)
-            a.turns[i] = std::pow(static_cast<double>(append->rope_theta), -static_cast<double>(i) / a.rotary_pairs) /
-                         6.283185307179586;
+        pk::rotary_turns(a, append->rope_theta);
         enqueue_paged(ctx, stream, ctx->stats.paged_append_calls, ctx->stats.paged_append_ns, [&](hipStream_t s) {
             launch_checked(pk::launch_paged_append(a, s), "paged append launch");
             ++ctx->stats.dispatches;

@@ -253,6 +253,9 @@ uint64_t prompt_scratch(const ModelArgs& m, const ModelLayer* layers, uint32_t t
 // through every layer, into the KV ring; advances state[0].
 hipError_t launch_prompt_chunk(PromptArgs a, const ModelLayer* layers, uint32_t tokens, uint32_t pos0,
                                hipStream_t stream);
+// One step of a batched generation (paged.hpp).
+struct BatchArgs;
+hipError_t launch_batch_step(PromptArgs a, const ModelLayer* layers, const BatchArgs& b, hipStream_t stream);
 // Embedding rows of tokens[state[0] + i], i < rows, into hidden_state + i * stride.
 hipError_t launch_embed(const ModelArgs& a, uint32_t rows, uint64_t stride, hipStream_t stream);
 

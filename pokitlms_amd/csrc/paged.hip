@@ -352,6 +352,19 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendArgs a) {
         float x[8], y[8];
         Row::load(src + head * HD + 8u * c0, x);
         Row::load(src + head * HD + 8u * c1, y);
+        if constexpr (T == T_F32) {
+            const uint64_t step = isq ? a.q_part : a.kv_part;
+            for (uint32_t k = 1; k < a.parts; ++k) {
+                float u[8], v[8];
+                Row::load(src + k * step + head * HD + 8u * c0, u);
+                Row::load(src + k * step + head * HD + 8u * c1, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] += u[e];
+                    y[e] += v[e];
+                }
+            }
+        }
         const float* w = isv ? nullptr : isq ? a.q_norm : a.k_norm;
         if (w) {
             float ss = 0.0f;
@@ -412,6 +425,11 @@ hipError_t append_hd(const PagedAppendArgs& a, hipStream_t s) {
 }
 
 }  // namespace
+
+void rotary_turns(PagedAppendArgs& a, float theta) {
+    for (uint32_t i = 0; i < a.rotary_pairs; ++i)
+        a.turns[i] = pow(static_cast<double>(theta), -static_cast<double>(i) / a.rotary_pairs) / 6.283185307179586;
+}
 
 size_t paged_plan_work_words(uint32_t requests, uint32_t max_tokens) {
     return requests <= kPlanThreads && max_tokens <= kPlanFusedTokens ? 0u : 2u * static_cast<size_t>(requests);

@@ -53,9 +53,14 @@ struct PagedAppendArgs {
     const uint32_t* positions;                            // [axes][position_stride]
     uint64_t position_stride;
     const uint32_t* slots;
+    // F32 rows as sums of `parts` partial ones (a projection's K split), in order, these
+    // strides apart
+    uint32_t parts;
+    uint64_t q_part, kv_part;
     double turns[kMaxRotaryPairs];    // theta^(-i / pairs) / 2 pi
     uint8_t axis[kMaxRotaryPairs];
 };
+void rotary_turns(PagedAppendArgs& a, float theta);
 hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t stream);
 
 // Attention over the pages (pk_hip_paged_attention).
@@ -76,5 +81,22 @@ struct PagedAttentionArgs {
 size_t paged_attention_work_floats(const PagedAttentionArgs& a);
 uint32_t paged_attention_launches(const PagedAttentionArgs& a);
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, float* work, hipStream_t stream);
+
+// One step of a batched generation (prompt.hip): `rows` rows of plan.requests slots, whose
+// selected ones get logits and a next token.  Device memory throughout.
+struct BatchArgs {
+    PagedPlanArgs plan;               // rows: max_tokens
+    PagedAppendArgs append;           // k, v, q and norms per layer
+    PagedAttentionArgs attention;
+    uint32_t rows, selected, head_batch;  // rows of logits per pass over the head
+    uint16_t* kv;                     // per layer K pages, then V pages
+    uint64_t layer_kv;                // elements of one of them
+    uint32_t *tokens, *row_tokens;    // every request's tokens, this step's rows'
+    const uint32_t* token_start;      // per request: where its tokens start
+    const uint32_t* slot_request;     // per slot: its request
+    const uint32_t* select;           // per selected row: row, request
+    uint32_t *zero, *flags;           // a zero word; non-finite logits, a refused plan
+    float *att, *normed, *logits, *head_work, *attention_work;
+};
 
 }  // namespace pk

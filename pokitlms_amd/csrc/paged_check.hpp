@@ -143,6 +143,7 @@ inline PagedCheck check_append(const pk_hip_paged_append* p, PagedAppendArgs& a)
     a.heads = p->heads;
     a.rotary_pairs = p->rotary_dim / 2u;
     a.axes = p->axes;
+    a.parts = 1u;
     a.eps = p->rms_eps;
     a.q = p->q;
     a.k = p->k;

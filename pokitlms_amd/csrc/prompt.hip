@@ -24,6 +24,7 @@
 #include "gemm_split.hpp"
 #include "kquant.hpp"
 #include "launch.hpp"
+#include "paged.hpp"
 #include "route.hpp"
 
 namespace pk {
@@ -250,6 +251,76 @@ __global__ void k_prompt_advance(uint32_t* state, uint32_t n) {
     if (threadIdx.x == 0u) state[0] += n;
 }
 
+// ---------------------------------------------------------------------------
+// Batched generation: rows of several requests (their lengths by the paged plan).
+
+// Row t's token: its request's token at the row's position, prompt or generated.
+__global__ __launch_bounds__(256) void k_batch_tokens(BatchArgs b) {
+    const uint32_t t = blockIdx.x * 256u + threadIdx.x;
+    if (t == 0u && b.plan.status[0]) atomicOr(b.flags + 1, 1u);
+    if (t >= b.rows) return;
+    const uint32_t slot = b.plan.token_request[t];
+    // a plan that was refused has no rows: token 0 stands in, the call fails at its end
+    b.row_tokens[t] = slot < b.plan.requests
+                          ? b.tokens[b.token_start[b.slot_request[slot]] + b.plan.positions[t]] : 0u;
+}
+
+// The dense GEMMs' operand of `chunks` runs of 32 values.
+__global__ __launch_bounds__(256) void k_prompt_split(const float* x, uint64_t chunks, uint16_t* parts, float* scales,
+                                                      float* sums) {
+    const uint64_t chunk = blockIdx.x * 8ull + threadIdx.x / 32u;
+    if (chunk >= chunks) return;  // half waves, whose lanes split_chunk keeps apart
+    split_chunk(x[chunk * 32u + (threadIdx.x & 31u)], threadIdx.x & 63u, chunk, parts, scales, sums);
+}
+
+// The selected rows, one after another.
+__global__ __launch_bounds__(256) void k_batch_gather(const float* x, BatchArgs b, uint32_t n) {
+    const float* from = x + static_cast<uint64_t>(b.select[2u * blockIdx.x]) * n;
+    for (uint32_t i = threadIdx.x; i < n; i += 256u) b.normed[static_cast<uint64_t>(blockIdx.x) * n + i] = from[i];
+}
+
+// The first maximum of each selected row's logits as its request's next token
+// (sample_token at temperature 0, src/qwen3_moe_runner.cpp:320-333); non-finite logits are
+// flagged, and token 0 stands in where every logit is NaN.
+__global__ __launch_bounds__(1024) void k_batch_argmax(BatchArgs b, uint32_t vocab) {
+    __shared__ float bv[16];
+    __shared__ uint32_t bi[16];
+    const uint32_t tid = threadIdx.x, row = b.select[2u * blockIdx.x], request = b.select[2u * blockIdx.x + 1u];
+    const float* logits = b.logits + static_cast<uint64_t>(blockIdx.x) * vocab;
+    float best = -INFINITY;
+    uint32_t at = 0xffffffffu;
+    bool bad = false;
+    auto merge = [&](float v, uint32_t i) {
+        if (v > best || (v == best && i < at)) {
+            best = v;
+            at = i;
+        }
+    };
+    for (uint32_t i = tid; i < vocab; i += 1024u) {
+        const float v = logits[i];
+        bad = bad || !isfinite(v);
+        merge(v, i);
+    }
+    for (uint32_t d = 32; d > 0; d >>= 1) merge(__shfl_xor(best, d), __shfl_xor(at, d));
+    if ((tid & 63u) == 0u) {
+        bv[tid >> 6] = best;
+        bi[tid >> 6] = at;
+    }
+    if (__any(bad) && (tid & 63u) == 0u) atomicOr(b.flags, 1u);
+    __syncthreads();
+    if (tid == 0u) {
+        for (uint32_t w = 1; w < 16u; ++w) merge(bv[w], bi[w]);
+        b.tokens[b.token_start[request] + b.plan.positions[row] + 1u] = at < vocab ? at : 0u;
+    }
+}
+
+void prompt_norm(const PromptArgs& a, uint32_t tokens, const float* d, uint32_t parts, const float* w, float* x, bool split,
+                 hipStream_t s) {
+    const uint32_t H = a.m.hidden;
+    hipLaunchKernelGGL(k_prompt_norm, dim3(tokens), dim3(256), 0, s, a.h, d, parts, static_cast<uint64_t>(tokens) * H, w, H,
+                       a.m.rms_eps, x, split ? a.op_parts : nullptr, a.op_scale, a.op_sums);
+}
+
 bool gemm_type(uint32_t t) {
     return t == T_Q4_K || t == T_Q5_K || t == T_Q6_K || t == T_Q8_0 || t == T_Q4_0 || t == T_Q4_1;
 }
@@ -359,29 +430,25 @@ uint64_t prompt_scratch(const ModelArgs& m, const ModelLayer* layers, uint32_t t
     return at;
 }
 
-hipError_t launch_prompt_chunk(PromptArgs a, const ModelLayer* layers, uint32_t tokens, uint32_t pos0,
-                               hipStream_t s) {
+namespace {
+
+// Every layer for `tokens` rows whose embeddings lie in a.h; attention(l, L, ready) takes q,
+// k and v of a layer to the split operand of the output projection.  The last layer's MoE
+// output (a.y) is left to be added.
+template <typename F>
+hipError_t chunk_layers(PromptArgs& a, const ModelLayer* layers, uint32_t tokens, hipStream_t s, F attention) {
     const ModelArgs& m = a.m;
     const uint32_t qd = m.heads * m.head_dim, kd = m.kv_heads * m.head_dim, H = m.hidden;
     hipError_t err;
-    a.tokens = tokens;
-    ModelArgs em = m;
-    em.hidden_state = a.h;
-    if ((err = launch_embed(em, tokens, m.hidden, s))) return err;
     // the tile list of the dense GEMMs: one for both, from the wider
     const uint32_t rows = dense_rows(tokens, qd + 2u * kd > H ? qd + 2u * kd : H);
     a.dense_tiles = (tokens + rows - 1u) / rows;
     hipLaunchKernelGGL(k_prompt_tiles, dim3(1), dim3(256), 0, s, tokens, rows == 64u ? 1u : 0u,
                        a.dense_tiles, a.d_tiles, a.d_tiles + a.dense_tiles, a.d_offsets, a.d_perm);
     const float* delta = nullptr;
-    auto norm = [&](const float* d, uint32_t parts, const float* w, float* x, bool split) {
-        hipLaunchKernelGGL(k_prompt_norm, dim3(tokens), dim3(256), 0, s, a.h, d, parts,
-                           static_cast<uint64_t>(tokens) * H, w, H, m.rms_eps, x,
-                           split ? a.op_parts : nullptr, a.op_scale, a.op_sums);
-    };
     for (uint32_t l = 0; l < m.layers; ++l) {
         const ModelLayer& L = layers[l];
-        norm(delta, 1u, L.attn_norm, nullptr, true);
+        prompt_norm(a, tokens, delta, 1u, L.attn_norm, nullptr, true, s);
         if (L.qkv) {  // q, k and v in one GEMM
             const uint32_t n = qd + 2u * kd;
             a.qkv_parts = k_parts_for(a.dense_tiles, n, H);
@@ -407,21 +474,10 @@ hipError_t launch_prompt_chunk(PromptArgs a, const ModelLayer* layers, uint32_t 
             if ((err = dense(a, L.attn_type, L.k, kd, H, k, a.qkv_parts, s))) return err;
             if ((err = dense(a, L.attn_type, L.v, kd, H, v, a.qkv_parts, s))) return err;
         }
-        const dim3 gq(m.heads + m.kv_heads, tokens), ga(m.heads, tokens);
-        const size_t lds = static_cast<size_t>(pos0 + tokens) * sizeof(float);
-#define PK_PA(HD)                                                                              \
-    case HD:                                                                                   \
-        hipLaunchKernelGGL(k_prompt_qk<HD>, gq, dim3(HD), 0, s, a, L);                         \
-        hipLaunchKernelGGL(k_prompt_attention<HD>, ga, dim3(256), lds, s, a, L);               \
-        break;
-        switch (m.head_dim) {
-            PK_PA(64) PK_PA(128) PK_PA(256)
-            default: return hipErrorInvalidValue;
-        }
-#undef PK_PA
+        if ((err = attention(l, L))) return err;
         const uint32_t op = k_parts_for(a.dense_tiles, H, qd);
         if ((err = dense(a, L.attn_type, L.o, H, qd, a.attn_out, op, s))) return err;
-        norm(a.attn_out, op, L.ffn_norm, a.x, false);
+        prompt_norm(a, tokens, a.attn_out, op, L.ffn_norm, a.x, false, s);
         MoePrefillArgs g = a.moe;
         g.layer = L.moe;
         g.tokens = tokens;
@@ -436,7 +492,87 @@ hipError_t launch_prompt_chunk(PromptArgs a, const ModelLayer* layers, uint32_t 
         if ((err = launch_prefill_down(g, s))) return err;
         delta = a.y;
     }
+    return hipSuccess;
+}
+
+}  // namespace
+
+hipError_t launch_prompt_chunk(PromptArgs a, const ModelLayer* layers, uint32_t tokens, uint32_t pos0,
+                               hipStream_t s) {
+    const ModelArgs& m = a.m;
+    hipError_t err;
+    a.tokens = tokens;
+    ModelArgs em = m;
+    em.hidden_state = a.h;
+    if ((err = launch_embed(em, tokens, m.hidden, s))) return err;
+    err = chunk_layers(a, layers, tokens, s, [&](uint32_t, const ModelLayer& L) -> hipError_t {
+        const dim3 gq(m.heads + m.kv_heads, tokens), ga(m.heads, tokens);
+        const size_t lds = static_cast<size_t>(pos0 + tokens) * sizeof(float);
+#define PK_PA(HD)                                                                              \
+    case HD:                                                                                   \
+        hipLaunchKernelGGL(k_prompt_qk<HD>, gq, dim3(HD), 0, s, a, L);                         \
+        hipLaunchKernelGGL(k_prompt_attention<HD>, ga, dim3(256), lds, s, a, L);               \
+        return hipSuccess;
+        switch (m.head_dim) {
+            PK_PA(64) PK_PA(128) PK_PA(256)
+            default: return hipErrorInvalidValue;
+        }
+#undef PK_PA
+    });
+    if (err != hipSuccess) return err;
     return launch_advance(m.state, tokens, s);
+}
+
+hipError_t launch_batch_step(PromptArgs a, const ModelLayer* layers, const BatchArgs& b, hipStream_t s) {
+    const ModelArgs& m = a.m;
+    const uint32_t rows = b.rows, H = m.hidden, qd = m.heads * m.head_dim;
+    hipError_t err;
+    a.tokens = rows;
+    if ((err = launch_paged_plan(b.plan, s))) return err;
+    hipLaunchKernelGGL(k_batch_tokens, dim3((rows + 255u) / 256u), dim3(256), 0, s, b);
+    ModelArgs em = m;
+    em.hidden_state = a.h;
+    em.tokens = b.row_tokens;
+    em.state = b.zero;
+    if ((err = launch_embed(em, rows, H, s))) return err;
+    PagedAppendArgs ap = b.append;
+    PagedAttentionArgs at = b.attention;
+    err = chunk_layers(a, layers, rows, s, [&](uint32_t l, const ModelLayer& L) -> hipError_t {
+        ap.kv.k = at.kv.k = b.kv + 2u * l * b.layer_kv;
+        ap.kv.v = at.kv.v = at.kv.k + b.layer_kv;
+        ap.q = a.q;
+        ap.k = a.k;
+        ap.v = a.v;
+        ap.q_stride = a.q_stride;
+        ap.k_stride = ap.v_stride = a.kv_stride;
+        ap.parts = a.qkv_parts;
+        ap.q_part = a.q_part;
+        ap.kv_part = a.kv_part;
+        ap.q_norm = L.q_norm;
+        ap.k_norm = L.k_norm;
+        ap.q_out = a.qr;
+        hipError_t e = launch_paged_append(ap, s);
+        if (e != hipSuccess) return e;
+        at.q = a.qr;
+        at.out = b.att;
+        if ((e = launch_paged_attention(at, b.attention_work, s))) return e;
+        const uint64_t chunks = static_cast<uint64_t>(rows) * qd / 32u;
+        hipLaunchKernelGGL(k_prompt_split, dim3(static_cast<uint32_t>((chunks + 7u) / 8u)), dim3(256), 0, s, b.att,
+                           chunks, a.op_parts, a.op_scale, a.op_sums);
+        return hipGetLastError();
+    });
+    if (err != hipSuccess || b.selected == 0u) return err;
+    // the selected rows' logits and the tokens after them
+    prompt_norm(a, rows, a.y, 1u, m.out_norm, a.x, false, s);
+    hipLaunchKernelGGL(k_batch_gather, dim3(b.selected), dim3(256), 0, s, a.x, b, H);
+    for (uint32_t i = 0; i < b.selected; i += b.head_batch) {
+        const uint32_t n = b.selected - i < b.head_batch ? b.selected - i : b.head_batch;
+        if ((err = launch_matvec(m.out_type, m.out, m.out_row, m.vocab, H, b.normed + static_cast<uint64_t>(i) * H,
+                                 b.logits + static_cast<uint64_t>(i) * m.vocab, n, s, b.head_work)))
+            return err;
+    }
+    hipLaunchKernelGGL(k_batch_argmax, dim3(b.selected), dim3(1024), 0, s, b, m.vocab);
+    return hipGetLastError();
 }
 
 hipError_t launch_advance(uint32_t* state, uint32_t n, hipStream_t s) {

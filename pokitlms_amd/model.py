@@ -189,6 +189,27 @@ class Qwen3MoeModel:
         stats = {k: getattr(st, k) for k, _ in st._fields_}
         return out[:n_new], logits, stats
 
+    def generate_batch(self, prompts, n_new, want_logits: bool = False):
+        """generate for many prompts at once over one paged KV cache (fast mode):
+        the new tokens per prompt, the logits after each prompt (or None) and the
+        stats.  n_new: one number for all, or one per prompt."""
+        ps = [np.ascontiguousarray(p, dtype=np.uint32).reshape(-1) for p in prompts]
+        counts = [int(n_new)] * len(ps) if np.ndim(n_new) == 0 else [int(n) for n in n_new]
+        if len(counts) != len(ps):
+            raise ValueError("n_new needs one number per prompt")
+        outs = [np.zeros(max(n, 1), np.uint32) for n in counts]
+        logits = [np.zeros(self.shape.vocab, np.float32) for _ in ps] if want_logits else None
+        reqs = (_abi.BatchRequest * max(len(ps), 1))(*[
+            _abi.BatchRequest(p.ctypes.data, p.size, n, o.ctypes.data,
+                              logits[i].ctypes.data if want_logits else None)
+            for i, (p, n, o) in enumerate(zip(ps, counts, outs))])
+        st = _abi.GenerationStats()
+        err = ctypes.create_string_buffer(_ERRBUF)
+        _raise(_abi.lib().pk_hip_qwen3moe_generate_batch(self.handle, reqs, len(ps),
+                                                         ctypes.byref(st), err, _ERRBUF), err)
+        stats = {k: getattr(st, k) for k, _ in st._fields_}
+        return [o[:n] for o, n in zip(outs, counts)], logits, stats
+
     def resident_bytes(self) -> int:
         return sum(w.nbytes for w in self.weights.values())
 
