@@ -155,6 +155,7 @@ class PagedPlan:
                                        new_lens, release or None, block_table, free_pages,
                                        free_count, lens_out, free_count_out, query_start,
                                        positions, slots, token_request, status)
+        self.ref = ctypes.byref(self.desc)
 
 
 class PagedAppend:
@@ -180,6 +181,7 @@ class PagedAppend:
             k_norm or None, positions or None, position_stride,
             None if axis is None else ctypes.addressof(axis), slots)
         self.desc.axis_map = axis  # lives as long as its address
+        self.ref = ctypes.byref(self.desc)
 
 
 def rotary_axes(sections, interleaved: bool = False) -> list:
@@ -214,6 +216,7 @@ class PagedAttention:
         self.desc = _abi.PagedAttentionDesc(cache.desc, gtype, heads, requests, max_tokens, max_new,
                                             table_stride, window, sinks, scale, q, out, q_stride,
                                             out_stride, query_start, lens, block_table)
+        self.ref = ctypes.byref(self.desc)
 
 
 class HipBackend:
@@ -584,19 +587,19 @@ class HipBackend:
     # ---- paged KV cache ---------------------------------------------------------------
     def paged_plan_async(self, plan: PagedPlan, stream: int = 0) -> None:
         """Pages, positions and slots of a step's new tokens (pk_hip_paged_plan_async)."""
-        status = self._plan(self.handle, plan.desc, stream or None, self._err, _ERRBUF)
+        status = self._plan(self.handle, plan.ref, stream or None, self._err, _ERRBUF)
         if status:
             _raise(status, self._err)
 
     def paged_append_async(self, append: PagedAppend, stream: int = 0) -> None:
         """Head norms, rotation and K and V into the pages (pk_hip_paged_append_async)."""
-        status = self._append(self.handle, append.desc, stream or None, self._err, _ERRBUF)
+        status = self._append(self.handle, append.ref, stream or None, self._err, _ERRBUF)
         if status:
             _raise(status, self._err)
 
     def paged_attention_async(self, attention: PagedAttention, stream: int = 0) -> None:
         """Attention of new tokens over the pages (pk_hip_paged_attention_async)."""
-        status = self._attend(self.handle, attention.desc, stream or None, self._err, _ERRBUF)
+        status = self._attend(self.handle, attention.ref, stream or None, self._err, _ERRBUF)
         if status:
             _raise(status, self._err)
 

@@ -185,6 +185,10 @@ struct pk_hip_ctx {
     // the paged cache's plans, and the parts of its attention's long rows
     DeviceBuffer<uint32_t> plan_work;
     DeviceBuffer<float> attn_work;
+    // the last append's angles per position: rotary_turns of this base and pair count
+    float turns_theta = 0.0f;
+    uint32_t turns_pairs = 0;
+    double turns[pk::kMaxRotaryPairs] = {};
     hipEvent_t ev[10] = {};
     int wall_rate_khz = 100000;  // wall_clock64() rate
 
@@ -2426,7 +2430,13 @@ pk_hip_status pk_hip_paged_append_async(pk_hip_ctx* ctx, const pk_hip_paged_appe
         require(pk::check_append(append, a));
         require_usable(ctx);
         std::lock_guard lock(ctx->mutex);
-        pk::rotary_turns(a, append->rope_theta);
+        if (a.rotary_pairs && (ctx->turns_pairs != a.rotary_pairs || ctx->turns_theta != append->rope_theta)) {
+            pk::rotary_turns(a, append->rope_theta);
+            std::copy_n(a.turns, a.rotary_pairs, ctx->turns);
+            ctx->turns_pairs = a.rotary_pairs;
+            ctx->turns_theta = append->rope_theta;
+        }
+        std::copy_n(ctx->turns, a.rotary_pairs, a.turns);
         enqueue_paged(ctx, stream, ctx->stats.paged_append_calls, ctx->stats.paged_append_ns, [&](hipStream_t s) {
             launch_checked(pk::launch_paged_append(a, s), "paged append launch");
             ++ctx->stats.dispatches;

@@ -336,9 +336,9 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendArgs a) {
     }
     __syncthreads();
     const uint32_t rows = a.heads + 2u * a.kv.kv_heads, l = tid % LP, rc = pairs / 8u;
-    // this lane's two chunks of eight values: rotation partners, or neighbours behind the rotated part
+    // this lane's two chunks of eight values: rotation partners, or one of each half of the rest
     const bool turned = l < rc;
-    const uint32_t c0 = turned ? l : 2u * l, c1 = turned ? l + rc : 2u * l + 1u;
+    const uint32_t c0 = turned ? l : l + rc, c1 = turned ? l + rc : l + LP;
     for (uint32_t i = tid / LP; i < NT * rows; i += ROWS) {
         const uint32_t t = t0 + i / rows, row = i % rows;
         if (t >= a.tokens) break;
