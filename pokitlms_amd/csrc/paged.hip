@@ -27,7 +27,7 @@ enum : uint32_t { PLAN_PAGES = 1, PLAN_TABLE = 2, PLAN_TOKENS = 4, PLAN_STATE = 
 
 constexpr uint32_t kPlanThreads = 1024;
 // Up to this many tokens one workgroup writes the slot map itself.
-constexpr uint32_t kPlanFusedTokens = 4096;
+constexpr uint32_t kPlanFusedTokens = 8192;
 
 struct PlanSums {
     uint32_t tokens, need, back;
@@ -50,37 +50,37 @@ __device__ __forceinline__ PlanSums wave_scan(PlanSums v) {
     return v;
 }
 
-// f(request, its table row, pages in use) for every released request, one wave each.
+// f(request, pages in use, lane) for every released request, a wave at a time; neighbours in
+// the table go to different waves.
 template <typename F>
 __device__ __forceinline__ void each_released(const PagedPlanArgs& a, uint32_t tid, F f) {
+    constexpr uint32_t WAVES = kPlanThreads / 64u;
     const uint32_t lane = tid & 63u, cap = a.table_stride << a.page_shift;
-    for (uint32_t base = tid & ~63u; base < a.requests; base += kPlanThreads) {
-        const uint32_t r = base + lane;
+    for (uint32_t base = tid >> 6; base < a.requests; base += kPlanThreads) {
+        const uint32_t r = base + WAVES * lane;
         const uint32_t len = r < a.requests && a.release[r] ? a.lens[r] : 0u;
         uint64_t todo = __ballot(len > 0u && len <= cap);
         while (todo) {
             const uint32_t l = static_cast<uint32_t>(__builtin_ctzll(todo));
             todo &= todo - 1u;
             const uint32_t n = __shfl(len, l);
-            f(base + l, (n + (1u << a.page_shift) - 1u) >> a.page_shift, lane);
+            f(base + WAVES * l, (n + (1u << a.page_shift) - 1u) >> a.page_shift, lane);
         }
     }
 }
 
-// Token t of request r: its position, its page (an old table entry, or the page popped
-// for it) and slot.  The first token of a fresh page writes the table entry.
-__device__ __forceinline__ void plan_token(const PagedPlanArgs& a, uint32_t t, uint32_t r, uint32_t len,
-                                           uint32_t j, uint32_t first, uint32_t top) {
-    const uint32_t mask = (1u << a.page_shift) - 1u, p = len + j, pi = p >> a.page_shift;
-    const uint32_t have = (len + mask) >> a.page_shift;
-    uint32_t* entry = a.table + static_cast<uint64_t>(r) * a.table_stride + pi;
-    uint32_t page;
-    if (pi < have) {
-        page = *entry;
-    } else {
-        page = a.free_pages[top - 1u - (first + pi - have)];
-        if ((p & mask) == 0u) *entry = page;
-    }
+// Row j of request r is its position p = len + j.  Its page is an old table entry or the one
+// popped for it: where that is read,
+__device__ __forceinline__ const uint32_t* plan_page(const PagedPlanArgs& a, uint32_t r, uint32_t len, uint32_t j,
+                                                     uint32_t first, uint32_t top) {
+    const uint32_t pi = (len + j) >> a.page_shift, have = (len + (1u << a.page_shift) - 1u) >> a.page_shift;
+    return pi < have ? a.table + static_cast<uint64_t>(r) * a.table_stride + pi : a.free_pages + (top - 1u - (first + pi - have));
+}
+// and what becomes of it: the first row of a fresh page writes the table entry.
+__device__ __forceinline__ void plan_token(const PagedPlanArgs& a, uint32_t t, uint32_t r, uint32_t len, uint32_t j,
+                                           uint32_t page) {
+    const uint32_t mask = (1u << a.page_shift) - 1u, p = len + j;
+    if ((p & mask) == 0u) a.table[static_cast<uint64_t>(r) * a.table_stride + (p >> a.page_shift)] = page;
     a.positions[t] = p;
     a.slots[t] = page < a.pages ? (page << a.page_shift) | (p & mask) : kNoSlot;
     a.token_request[t] = r;
@@ -236,13 +236,31 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PagedPlanArgs a) {
     }
     if constexpr (FUSED) {
         __syncthreads();
-        for (uint32_t t = tid; t < a.max_tokens; t += kPlanThreads) {
-            if (t >= tokens) {
-                plan_no_token(a, t);
-                continue;
+        // four tokens a thread at a time: their searches and page reads wait together
+        constexpr uint32_t U = 4u;
+        uint32_t widest = 1u;
+        while (2u * widest < R) widest *= 2u;
+        for (uint32_t t0 = tid; t0 < a.max_tokens; t0 += U * kPlanThreads) {
+            uint32_t r[U], page[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) r[u] = 0u;
+            for (uint32_t step = R > 1u ? widest : 0u; step > 0u; step /= 2u)
+#pragma unroll
+                for (uint32_t u = 0; u < U; ++u) {
+                    const uint32_t next = r[u] + step;
+                    if (next < R && s_start[next] <= t0 + u * kPlanThreads) r[u] = next;
+                }
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t t = t0 + u * kPlanThreads;
+                page[u] = t < tokens ? *plan_page(a, r[u], s_len[r[u]], t - s_start[r[u]], s_first[r[u]], top) : kNoSlot;
             }
-            const uint32_t r = plan_search(s_start, 0u, R - 1u, t);
-            plan_token(a, t, r, s_len[r], t - s_start[r], s_first[r], top);
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t t = t0 + u * kPlanThreads;
+                if (t < tokens) plan_token(a, t, r[u], s_len[r[u]], t - s_start[r[u]], page[u]);
+                else if (t < a.max_tokens) plan_no_token(a, t);
+            }
         }
     }
 }
@@ -263,7 +281,8 @@ __global__ __launch_bounds__(256) void k_paged_slots(PagedPlanArgs a) {
         return;
     }
     const uint32_t r = plan_search(a.query_start, lo, hi, t), start = a.query_start[r];
-    plan_token(a, t, r, a.lens_out[r] - (a.query_start[r + 1u] - start), t - start, a.work[r], top);
+    const uint32_t len = a.lens_out[r] - (a.query_start[r + 1u] - start);
+    plan_token(a, t, r, len, t - start, *plan_page(a, r, len, t - start, a.work[r], top));
 }
 
 // ---------------------------------------------------------------------------
