@@ -577,6 +577,113 @@ def test_steps_together_in_a_graph(hip):
         assert torch.all(out[t:] == 5.0)
 
 
+def test_attention_replayed_with_other_lengths(hip):
+    """A captured call of long contexts, replayed with other lengths, values and eager calls of
+    other shapes in between: each replay against a fresh eager call."""
+    cases = [attention_case(40 + i, lens, new, 8, 2, 128, "F32", "F16", 16, width_more=700 - max(lens) // 16)
+             for i, (lens, new) in enumerate((([9000, 40, 700], [1, 30, 2]), ([33, 10900, 1], [33, 1, 1]),
+                                              ([1, 64, 8000], [0, 1, 34]), ([9000, 5000, 7000], [1, 1, 1])))]
+    pages, rows = max(c["pages"] for c in cases), max(c["rows"] for c in cases)
+    width = max(c["table"].shape[1] for c in cases)
+    one = {**cases[0], "pages": pages, "rows": rows, "table": np.full((3, width), P.NONE, np.uint32),
+           "k": torch.zeros(pages, 16, 2, 128, dtype=torch.float16, device="cuda"),
+           "v": torch.zeros(pages, 16, 2, 128, dtype=torch.float16, device="cuda"),
+           "q": torch.zeros(rows, 8, 128, device="cuda")}
+    out = torch.zeros_like(one["q"])
+    call = attention_call(one, out)
+    lens, start, table = call.held
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    hip.paged_attention_async(call, stream.cuda_stream)  # sizes the scratch
+    hip.sync(stream.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        hip.paged_attention_async(call, torch.cuda.current_stream().cuda_stream)
+    other = attention_case(50, [5000, 6000], [1, 60], 4, 1, 64, "F16", "F16", 8)
+    for c in cases + cases[:2]:
+        one["k"][:c["pages"]], one["v"][:c["pages"]], one["q"][:c["rows"]] = c["k"], c["v"], c["q"]
+        lens.copy_(ints(c["lens"]))
+        start.copy_(ints(c["start"]))
+        full = np.full((3, width), P.NONE, np.uint32)
+        full[:, :c["table"].shape[1]] = c["table"]
+        table.copy_(ints(full))
+        out.fill_(5.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(c, out[:c["rows"]].contiguous())
+        assert torch.all(out[c["rows"]:] == 5.0)
+        run_attention(hip, other)
+
+
+def test_capture_refuses_scratch_growth(hip):
+    """A fresh context's first call under capture would need scratch: refused, and the context
+    still works."""
+    from pokitlms_amd.backend import HipBackend
+    c = attention_case(60, [9000, 300], [1, 2], 4, 2, 64, "F16", "F16", 16)
+    want = run_attention(hip, c)
+    with HipBackend(0) as fresh:
+        out = torch.full_like(c["q"], 5.0)
+        call = attention_call(c, out)
+        stream, refused = torch.cuda.Stream(), None
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            try:
+                fresh.paged_attention_async(call, torch.cuda.current_stream().cuda_stream)
+            except ValueError as e:
+                refused = str(e)
+        assert refused is not None and "outside stream capture" in refused
+        fresh.paged_attention_async(call, stream.cuda_stream)
+        fresh.sync(stream.cuda_stream)
+        assert torch.equal(out, want)
+
+
+def test_offsets_beyond_32_bits(hip):
+    """A cache of 9 GB whose pages lie 128 KB apart, K and V of a page side by side."""
+    pages, stride, page, kvh, dim = 70000, 1 << 16, 16, 2, 128
+    pool = torch.empty(pages * stride, dtype=torch.float16, device="cuda")
+    assert pages * stride > 1 << 32
+    g = np.random.default_rng(1)
+    table = np.full((2, 8), P.NONE, np.uint32)
+    table[0, :6], table[1, :2] = [69999, 3, 66000, 65537, 69990, 32769], [68001, 1]
+    lens, new = [90, 20], [25, 1]
+    for rows in (new, [1, 20]):
+        tokens = sum(rows)
+        qkv = torch.randn(sum(lens), 2 * kvh * dim, device="cuda", dtype=torch.float16)
+        slots = np.concatenate([table[r, np.arange(n) // page].astype(np.int64) * page + np.arange(n) % page
+                                for r, n in enumerate(lens)])
+        kv = PagedKV(pool.data_ptr(), pool.data_ptr() + stride, 1, pages, page, kvh, dim, stride, kvh * dim, dim)
+        at = ints(slots)
+        hip.paged_append_async(PagedAppend(kv, 1, len(slots), 0, k=qkv.data_ptr(), v=qkv[:, kvh * dim:].data_ptr(),
+                                           k_stride=2 * kvh * dim, v_stride=2 * kvh * dim, slots=at.data_ptr()))
+        q = torch.randn(tokens, 4, dim, device="cuda", dtype=torch.float16)
+        out = torch.full_like(q, 5.0)
+        ln, st, tb = ints(lens), ints(np.concatenate([[0], np.cumsum(rows)])), ints(table)
+        hip.paged_attention_async(PagedAttention(kv, 1, 4, 2, tokens, q=q.data_ptr(), out=out.data_ptr(),
+                                                 query_start=st.data_ptr(), lens=ln.data_ptr(),
+                                                 block_table=tb.data_ptr(), table_stride=8))
+        torch.cuda.synchronize()
+        small = {int(p): i for i, p in enumerate(np.unique(table[table != P.NONE]))}
+        k, v = np.zeros((len(small), page, kvh, dim)), np.zeros((len(small), page, kvh, dim))
+        x = f64(qkv)
+        for i, s in enumerate(slots):
+            k[small[int(s) // page], s % page] = x[i, :kvh * dim].reshape(kvh, dim)
+            v[small[int(s) // page], s % page] = x[i, kvh * dim:].reshape(kvh, dim)
+        near = np.vectorize(lambda p: small.get(int(p), P.NONE))(table).astype(np.uint32)
+        want, bound = P.attention(f64(q), k, v, near, np.concatenate([[0], np.cumsum(rows)]), lens, page,
+                                  dim ** -0.5, 0, 0)
+        tol = P.attention_tolerance(want, bound, dim, "F16", "F16")
+        assert np.all(np.abs(f64(out) - want) <= tol)
+
+
+def test_lengths_past_the_table_count_as_its_end(hip):
+    c = attention_case(61, [64, 30], [5, 1], 4, 2, 64, "F16", "F16", 16, width_more=0)
+    want = run_attention(hip, c)
+    got = run_attention(hip, {**c, "lens": [0xFFFFFFFF, 30]})
+    assert torch.equal(got, want)
+
+
 def test_two_contexts_on_two_streams(hip):
     """The same work in flight on two contexts' streams at once."""
     from pokitlms_amd.backend import HipBackend
