@@ -224,9 +224,22 @@ __device__ __forceinline__ void write_head(const PagedAttentionArgs& a, const Ro
     h[1] = u32x4{p.slot, 0u, 0u, 0u};
 }
 
+// Whether any of a lane's sums is NaN.
+template <uint32_t N, typename V>
+__device__ __forceinline__ bool any_nan(const V (&o)[N]) {
+    constexpr uint32_t W = sizeof(V) / sizeof(float);
+    bool nan = false;
+#pragma unroll
+    for (uint32_t d = 0; d < N; ++d)
+#pragma unroll
+        for (uint32_t x = 0; x < W; x += 2) nan = nan || __builtin_isunordered(o[d][x], o[d][x + 1]);
+    return nan;
+}
+
 // One row over the key tiles t0 .. t1 - 1 by one wave, reading only what the row sees: for
-// rows into which a masked value (NaN or infinite, with weight 0) has come by way of a
-// tile whose other rows see it.
+// rows into which a masked value (NaN or infinite, with weight 0) may have come by way of a
+// tile whose other rows see it, that is, whose sums turned NaN in a tile of which they see
+// a part.
 __device__ void row_alone(const PagedAttentionArgs& a, const Piece& p, const KeyTiles& keys, uint32_t kt, uint32_t t0,
                           uint32_t t1, uint32_t hk, uint32_t f, const RowTo& to) {
     const uint32_t lane = threadIdx.x & 63u, HD = a.kv.head_dim, token = p.q0 + a.group(f);
@@ -442,6 +455,7 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
 #pragma unroll
     for (uint32_t e = 0; e < DPL; ++e) o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
+    bool suspect = false;
     uint32_t b = b0 + wave, next_page = kNoSlot;
     if (b < b1) {
         place(b, entry(b));
@@ -468,8 +482,10 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
         }
         __builtin_amdgcn_sched_barrier(0);
         // every row sees the whole tile, or each score asks
-        if (here != 0xffffffffu || static_cast<int32_t>(base + KT) - 1 > p_first ||
-            (a.window && base + a.window <= static_cast<uint32_t>(p_last) && base + KT > a.sinks)) {
+        const bool cut = here != 0xffffffffu || static_cast<int32_t>(base + KT) - 1 > p_first ||
+                         (a.window && base + a.window <= static_cast<uint32_t>(p_last) && base + KT > a.sinks);
+        const bool watch = cut && p_first != p_last && !any_nan(o);
+        if (cut) {
 #pragma unroll
             for (uint32_t t = 0; t < 2; ++t)
 #pragma unroll
@@ -515,6 +531,7 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
         }
         if (more) load_v();
         __builtin_amdgcn_sched_barrier(0);
+        if (cut && p_first != p_last) suspect = suspect || (watch && any_nan(o));
     }
     // the four waves' parts
     l += __shfl_xor(l, 16u);
@@ -523,7 +540,8 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
         lds.m[wave][j] = m;
         lds.l[wave][j] = l;
     }
-    __syncthreads();
+    __syncthreads();  // lds.bad is 0 as well
+    if (suspect && j < rows && l == l) atomicOr(&lds.bad, 1u << j);
     {
         const float mm = fmaxf(fmaxf(lds.m[0][j], lds.m[1][j]), fmaxf(lds.m[2][j], lds.m[3][j]));
         const float keep = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mm);
@@ -540,24 +558,17 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
     float sum = 0.0f;
 #pragma unroll
     for (uint32_t v = 0; v < 4; ++v) sum += mm == -INFINITY ? lds.l[v][row] : lds.l[v][row] * __builtin_amdgcn_exp2f(lds.m[v][row] - mm);
-    f32x4 r[HD / 64u];
-    bool bad = false;
-#pragma unroll
-    for (uint32_t k = 0; k < HD / 64u; ++k) {
-        const uint32_t d = 64u * k + 4u * (tid % 16u);
-        r[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (uint32_t v = 0; v < 4; ++v) r[k] = r[k] + *reinterpret_cast<const f32x4*>(&lds.o[v][row][d]);
-#pragma unroll
-        for (uint32_t x = 0; x < 4; ++x) bad = bad || r[k][x] != r[k][x];
-    }
-    if (bad && row < rows) atomicOr(&lds.bad, 1u << row);
-    __syncthreads();
-    const uint32_t again = p_first != p_last ? lds.bad : 0u;
+    const uint32_t again = lds.bad;
     if (row < rows && !((again >> row) & 1u)) {
         const RowTo to = row_to(a, w, p, BM, hk, row);
 #pragma unroll
-        for (uint32_t k = 0; k < HD / 64u; ++k) store_row4(a, to, 64u * k + 4u * (tid % 16u), r[k], mm, sum);
+        for (uint32_t k = 0; k < HD / 64u; ++k) {
+            const uint32_t d = 64u * k + 4u * (tid % 16u);
+            f32x4 r = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (uint32_t v = 0; v < 4; ++v) r = r + *reinterpret_cast<const f32x4*>(&lds.o[v][row][d]);
+            store_row4(a, to, d, r, mm, sum);
+        }
     }
     if (again)
         for (uint32_t i = wave; i < rows; i += 4u)
@@ -700,6 +711,7 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
 #pragma unroll
         for (uint32_t x = 0; x < 16; ++x) o[d][x] = 0.0f;
     float m = -INFINITY, l = 0.0f;
+    bool suspect = false;
     uint64_t next_there = 0;
     uint32_t page = kNoSlot;
     if (t0 < t1) {
@@ -741,8 +753,10 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, 6u * NP, 0);
-        if (there != ~0ull || static_cast<int32_t>(base + KT) - 1 > w_first ||
-            (a.window && base + a.window <= static_cast<uint32_t>(w_last) && base + KT > a.sinks)) {
+        const bool cut = there != ~0ull || static_cast<int32_t>(base + KT) - 1 > w_first ||
+                         (a.window && base + a.window <= static_cast<uint32_t>(w_last) && base + KT > a.sinks);
+        const bool watch = cut && w_first != w_last && !any_nan(o);
+        if (cut) {
             const uint64_t mine = there >> (4u * h);
 #pragma unroll
             for (uint32_t ks = 0; ks < 2; ++ks)
@@ -788,15 +802,11 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
                     for (uint32_t i = 0; i < NP; ++i) o[d] = M::mma32(__builtin_bit_cast(V8, x), pp[i], o[d]);
                 }
             }
+        if (cut && w_first != w_last) suspect = suspect || (watch && any_nan(o));
     }
     if (!wave_live) return;
     l += __shfl_xor(l, 32u);
-    bool bad = false;
-#pragma unroll
-    for (uint32_t d = 0; d < DT; ++d)
-#pragma unroll
-        for (uint32_t x = 0; x < 16; ++x) bad = bad || o[d][x] != o[d][x];
-    uint64_t again = w_first != w_last ? __ballot(bad && live) : 0u;
+    uint64_t again = __ballot(suspect && live && l == l);
     again = (again | (again >> 32)) & 0xffffffffu;
     if (live && !((again >> j) & 1u)) {
         const RowTo to = row_to(a, w, p, BM, hk, 32u * wave + j);

@@ -402,6 +402,45 @@ def test_attention_masked_values_do_not_matter(hip, gtype, cache):
     assert np.all(np.abs(f64(got) - want)[rows] <= tol[rows])
 
 
+def test_attention_nan_that_rows_see_costs_no_more(hip):
+    """A NaN key, value or query makes NaN of the rows that see it, and of no others, in the time
+    that any values take."""
+    import time
+    c = attention_case(62, [4000, 4000], [4000, 1], 8, 2, 128, "BF16", "BF16", 16)
+    run_attention(hip, c)
+    def timed(case):
+        run_attention(hip, case)
+        t = time.perf_counter()
+        out = run_attention(hip, case)
+        return out, time.perf_counter() - t
+    clean, plain = timed(c)
+    def at(r, i):
+        return int(c["table"][r, i // 16]), i % 16
+    for name in ("k", "v"):
+        bad = {**c, name: c[name].clone()}
+        bad[name][at(0, 100)][0, 5] = float("nan")
+        bad[name][at(1, 100)][1, 5] = float("nan")
+        got, spent = timed(bad)
+        nan = torch.isnan(got)
+        seen = nan[100:4000, :4] if name == "k" else nan[100:4000, :4, 5]
+        assert seen.all() and nan[4000, 4:, 5].all()
+        nan[100:4000, :4] = False
+        nan[4000, 4:] = False
+        assert not nan.any() and torch.equal(got[:64], clean[:64]) and torch.equal(got[:100, 4:], clean[:100, 4:])
+        # rows of the tile that holds the NaN without seeing it are done again by themselves, with
+        # unrounded weights: half a step of BF16 of max |v| (2^-12 more for FP32's sums), and
+        # each side's own rounding
+        off = (got[64:100, :4].float() - clean[64:100, :4].float()).abs()
+        vmax = c["v"][torch.isfinite(c["v"])].abs().max().float()
+        assert torch.all(off <= vmax * (2.0 ** -8 + 2.0 ** -12) + clean[64:100, :4].float().abs() * 2.0 ** -7)
+        assert spent < 20 * plain + 0.05
+    bad = {**c, "q": c["q"].clone()}
+    bad["q"][77, 3, 9] = float("nan")
+    got, spent = timed(bad)
+    nan = torch.isnan(got)
+    assert nan[77, 3].all() and nan.sum() == 128 and spent < 20 * plain + 0.05
+
+
 @pytest.mark.parametrize("scale", (0.3, 1e-8))
 def test_attention_scale_and_large_scores(hip, scale):
     c = attention_case(9, [90, 33], [30, 1], 4, 2, 64, "F32", "F16", 16)
