@@ -85,7 +85,15 @@ struct RowWork {
     float* part;
     uint32_t* head;   // per split tile kHeadWords: parts, first row's q row, tokens, tile, first part's place
     uint32_t* count;  // [1]
+    // of more than kWaveRequests requests: k_paged_schedule's pieces and split tiles, then per
+    // request its first unit and its first part and split tile (null: every wave counts)
+    uint32_t* schedule;
 };
+// Counted by every wave, or by a launch before (single tokens of 32 heads over 4 of 128, 200
+// positions each): 65 requests 10.5 us or 13.8, 128 16.0 or 19.2, 193 28.4 or 26.9, 256 31.7 or
+// 29.8, 1024 262 or 111, 8192 (100 positions) 14,525 or 587.
+constexpr uint32_t kWaveRequests = 192u;
+constexpr uint32_t schedule_words(uint32_t requests) { return 4u + 2u * (requests + 1u); }
 
 // One workgroup's piece: part `part` of `parts` of row tile `tile` of request r; its place
 // among the parts and its tile's among the split tiles, both per kv head.
@@ -108,66 +116,162 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {  // inclusive sums
     return v;
 }
 
-// The piece of unit u, from the lengths alone: every wave finds it by itself, its lanes
-// taking a 64th of the requests each (exclusive sums give each request its units).  splits:
-// split tiles per kv head.
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, uint32_t lane) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), static_cast<int>(lane)));
+}
+
+// A request's rows and work, from the lengths.
+struct Request {
+    uint32_t q0, q1, len;
+    RequestWork work;
+};
+__device__ __forceinline__ Request request_of(const PagedAttentionArgs& a, const RowWork& w, uint32_t bm, uint32_t r) {
+    const uint32_t at = r < a.requests ? r : 0u, positions = a.table_stride << a.kv.page_shift;
+    Request q{a.query_start[at], a.query_start[at + 1u], a.lens[at], {0u, 0u}};
+    const uint32_t fresh = r < a.requests ? paged_new(q.q0, q.q1, a.max_new, a.max_tokens) : 0u;
+    q.work = request_work(fresh, q.len, a.group, bm, w.min_rows, w.max_rows, a.window, a.sinks, positions);
+    return q;
+}
+// Its units, and its parts of split tiles and split tiles in one word (over all requests at
+// most 2 * target and target).
+__device__ __forceinline__ uint32_t units_of(const RequestWork& q, uint32_t pieces, uint32_t& cut) {
+    const uint32_t n = request_parts(q.keys, pieces);
+    cut = n > 1u ? q.tiles * (n + 0x10000u) : 0u;
+    return q.tiles * n;
+}
+
+// The piece of unit u.  Up to kWaveRequests every wave finds it by itself from the lengths,
+// its lanes taking a 64th of the requests each: exclusive sums give each its units.  With
+// more, a launch before has left those sums, and two looks of 64 lanes find the request.
+// splits: split tiles per kv head.
 __device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, const RowWork& w, uint32_t bm, uint32_t u,
                                            Piece& p, uint32_t& splits) {
-    const uint32_t lane = threadIdx.x & 63u, per = (a.requests + 63u) / 64u;
-    const uint32_t positions = a.table_stride << a.kv.page_shift;
-    uint32_t q0, q1, len;  // of the request asked for last
-    auto work_of = [&](uint32_t r) -> RequestWork {
-        const uint32_t at = r < a.requests ? r : 0u;
-        q0 = a.query_start[at];
-        q1 = a.query_start[at + 1u];
-        len = a.lens[at];
-        const uint32_t fresh = r < a.requests ? paged_new(q0, q1, a.max_new, a.max_tokens) : 0u;
-        return request_work(fresh, len, a.group, bm, w.min_rows, w.max_rows, a.window, a.sinks, positions);
-    };
-    RequestWork one = work_of(lane * per);
-    double work = static_cast<double>(one.tiles) * one.keys;  // exact below 2^53
-    for (uint32_t i = 1; i < per; ++i) {
-        one = work_of(lane * per + i);
-        work += static_cast<double>(one.tiles) * one.keys;
+    const uint32_t lane = threadIdx.x & 63u, positions = a.table_stride << a.kv.page_shift;
+    Request q;
+    uint32_t pieces, left, before;
+    if (!w.schedule) {
+        const uint32_t per = (a.requests + 63u) / 64u;
+        q = request_of(a, w, bm, lane * per);
+        double work = static_cast<double>(q.work.tiles) * q.work.keys;  // exact below 2^53
+        for (uint32_t i = 1; i < per; ++i) {
+            q = request_of(a, w, bm, lane * per + i);
+            work += static_cast<double>(q.work.tiles) * q.work.keys;
+        }
+        work = lane63(group_sum<64>(work));
+        pieces = part_pieces(static_cast<uint64_t>(work) * a.kv.kv_heads, w.log_target, w.least);
+        uint32_t units = 0u, cut = 0u, c;
+        for (uint32_t i = 0; i < per; ++i) {
+            if (per > 1u) q = request_of(a, w, bm, lane * per + i);
+            units += units_of(q.work, pieces, c);
+            cut += c;
+        }
+        uint32_t eu = wave_prefix(units), ec = wave_prefix(cut);
+        splits = lane_value(ec, 63u) >> 16;
+        eu -= units;
+        ec -= cut;
+        const uint64_t mine = __ballot(u >= eu && u - eu < units);
+        if (!mine) return false;
+        uint32_t r = lane * per;
+        left = u - eu;
+        for (uint32_t i = 0; per > 1u && i < per; ++i) {  // only the owner's walk matters
+            q = request_of(a, w, bm, lane * per + i);
+            r = lane * per + i;
+            const uint32_t n = units_of(q.work, pieces, c);
+            if (left < n || i + 1u == per) break;
+            left -= n;
+            ec += c;
+        }
+        const uint32_t owner = static_cast<uint32_t>(__builtin_ctzll(mine));
+        p.r = lane_value(r, owner);
+        left = lane_value(left, owner);
+        before = lane_value(ec, owner);
+        q.q0 = lane_value(q.q0, owner);
+        q.q1 = lane_value(q.q1, owner);
+        q.len = lane_value(q.len, owner);
+        q.work = {lane_value(q.work.tiles, owner), lane_value(q.work.keys, owner)};
+    } else {
+        const uint32_t R = a.requests, step = (R + 63u) / 64u;
+        const uint32_t *start = w.schedule + 4u, *cuts = start + R + 1u;
+        pieces = w.schedule[0];
+        splits = w.schedule[1];
+        // the last request that starts at u or before
+        const uint32_t at = lane * step < R ? lane * step : R;
+        const uint32_t k = static_cast<uint32_t>(__popcll(__ballot(at < R && start[at] <= u))) - 1u;
+        if (u >= start[R]) return false;
+        const uint32_t base = k * step;
+        uint32_t count = 0;
+        for (uint32_t i = 0; i < step; i += 64u) {
+            const uint32_t r = base + i + lane;
+            count += static_cast<uint32_t>(__popcll(__ballot(i + lane < step && r < R && start[r < R ? r : R] <= u)));
+        }
+        p.r = base + count - 1u;
+        left = u - start[p.r];
+        before = cuts[p.r];
+        q = request_of(a, w, bm, p.r);
     }
-    work = lane63(group_sum<64>(work));
+    p.parts = request_parts(q.work.keys, pieces);
+    p.tile = q.work.tiles - 1u - left / p.parts;  // the tiles that see most keys first
+    p.part = left % p.parts;
+    p.slot = (before & 0xffffu) + left;
+    p.split = (before >> 16) + left / p.parts;
+    p.q0 = q.q0;
+    p.fresh = q.q1 - q.q0;
+    p.len = static_cast<int32_t>(q.len < positions ? q.len : positions);
+    return true;
+}
+
+// What find_piece needs where there are more requests than lanes: a workgroup per kind of
+// tile, its threads a 1024th of the requests each.
+__global__ __launch_bounds__(1024) void k_paged_schedule(PagedAttentionArgs a, RowWork few, RowWork many) {
+    __shared__ double s_work[16];
+    __shared__ uint32_t s_units[16], s_cut[16];
+    const RowWork& w = blockIdx.x ? many : few;
+    const uint32_t bm = blockIdx.x ? 128u : 16u, R = a.requests;
+    if (!w.schedule) return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, per = (R + 1023u) / 1024u;
+    double work = 0.0;
+    for (uint32_t i = 0; i < per; ++i) {
+        const RequestWork q = request_of(a, w, bm, tid * per + i).work;
+        work += static_cast<double>(q.tiles) * q.keys;
+    }
+    work = group_sum<64>(work);
+    if (lane == 63u) s_work[wave] = work;
+    __syncthreads();
+    work = 0.0;
+    for (uint32_t i = 0; i < 16u; ++i) work += s_work[i];
     const uint32_t pieces = part_pieces(static_cast<uint64_t>(work) * a.kv.kv_heads, w.log_target, w.least);
-    // units, and parts and split tiles in one word (at most 2 * target, target)
     uint32_t units = 0u, cut = 0u;
     for (uint32_t i = 0; i < per; ++i) {
-        if (per > 1u) one = work_of(lane * per + i);
-        const uint32_t n = request_parts(one.keys, pieces);
-        units += one.tiles * n;
-        cut += n > 1u ? one.tiles * (n + 0x10000u) : 0u;
+        uint32_t c;
+        units += units_of(request_of(a, w, bm, tid * per + i).work, pieces, c);
+        cut += c;
     }
     uint32_t eu = wave_prefix(units), ec = wave_prefix(cut);
-    splits = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ec), 63)) >> 16;
+    if (lane == 63u) {
+        s_units[wave] = eu;
+        s_cut[wave] = ec;
+    }
+    __syncthreads();
     eu -= units;
     ec -= cut;
-    const uint64_t mine = __ballot(u >= eu && u - eu < units);
-    if (!mine) return false;
-    uint32_t r = lane * per, left = u - eu;
-    for (uint32_t i = 0; per > 1u && i < per; ++i) {  // only the owner's walk matters
-        one = work_of(lane * per + i);
-        const uint32_t n = request_parts(one.keys, pieces);
-        r = lane * per + i;
-        if (left < one.tiles * n || i + 1u == per) break;
-        left -= one.tiles * n;
-        ec += n > 1u ? one.tiles * (n + 0x10000u) : 0u;
+    for (uint32_t i = 0; i < wave; ++i) {
+        eu += s_units[i];
+        ec += s_cut[i];
     }
-    const int owner = __builtin_ctzll(mine);
-    auto get = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), owner)); };
-    const uint32_t tiles = get(one.tiles), at = get(left), before = get(ec), n = get(len);
-    p.r = get(r);
-    p.parts = request_parts(get(one.keys), pieces);
-    p.tile = tiles - 1u - at / p.parts;  // the tiles that see most keys first
-    p.part = at % p.parts;
-    p.slot = (before & 0xffffu) + at;
-    p.split = (before >> 16) + at / p.parts;
-    p.q0 = get(q0);
-    p.fresh = get(q1) - p.q0;
-    p.len = static_cast<int32_t>(n < positions ? n : positions);
-    return true;
+    uint32_t *start = w.schedule + 4u, *cuts = start + R + 1u;
+    for (uint32_t i = 0; i < per && tid * per + i < R; ++i) {
+        const uint32_t r = tid * per + i;
+        uint32_t c;
+        start[r] = eu;
+        cuts[r] = ec;
+        eu += units_of(request_of(a, w, bm, r).work, pieces, c);
+        ec += c;
+    }
+    if (tid == 1023u) {  // behind every request's
+        start[R] = eu;
+        w.schedule[0] = pieces;
+        w.schedule[1] = ec >> 16;
+    }
 }
 
 // 4 values of a row of q's type.
@@ -1012,6 +1116,9 @@ struct Half {
     uint32_t target() const { return 1u << w.log_target; }
     uint64_t part_floats() const { return splits ? most_parts(target()) * bm : 0u; }
     uint64_t words() const { return splits ? target() * kHeadWords + 4u : 0u; }  // a split tile has two parts
+    uint32_t schedule_words(uint32_t requests) const {
+        return used && requests > kWaveRequests ? (pk::schedule_words(requests) + 3u) / 4u * 4u : 0u;
+    }
     uint64_t units(uint32_t kv_heads) const { return most_units(tiles / kv_heads, kv_heads, splits ? target() : 0u) * kv_heads; }
     uint32_t split_tiles() const { return !splits ? 0u : tiles < target() ? static_cast<uint32_t>(tiles) : target(); }
 };
@@ -1022,10 +1129,10 @@ void halves(const PagedAttentionArgs& a, Half& few, Half& many) {
     // a request of the 16-row tiles has at most kFewRows rows
     const uint64_t n = a.requests < a.max_tokens ? a.requests : a.max_tokens;
     const uint64_t tokens = n * (kFewRows / group ? kFewRows / group : 1u);
-    few = Half{{1u, kFewRows, kRowsTarget, kLeast, nullptr, nullptr, nullptr}, 16u, group <= kFewRows, false,
+    few = Half{{1u, kFewRows, kRowsTarget, kLeast, nullptr, nullptr, nullptr, nullptr}, 16u, group <= kFewRows, false,
                most_tiles(tokens < a.max_tokens ? tokens : a.max_tokens, a.requests, group, 16u) * a.kv.kv_heads};
     if (few.tiles < kFewTiles) few.w.log_target = kFewTilesTarget;
-    many = Half{{kFewRows + 1u, 0xffffffffu, kTilesTarget, kLeast, nullptr, nullptr, nullptr}, kTileRows,
+    many = Half{{kFewRows + 1u, 0xffffffffu, kTilesTarget, kLeast, nullptr, nullptr, nullptr, nullptr}, kTileRows,
                 static_cast<uint64_t>(a.max_new) * group > kFewRows, false,
                 most_tiles(a.max_tokens, a.requests, group, kTileRows) * a.kv.kv_heads};
     few.splits = may_split && few.used;
@@ -1037,6 +1144,8 @@ hipError_t attention_t(const PagedAttentionArgs& a, const Half& few, const Half&
     const uint64_t fu = few.used ? few.units(a.kv.kv_heads) : 0u, mu = many.used ? many.units(a.kv.kv_heads) : 0u;
     if (fu + mu >= (1ull << 31)) return hipErrorInvalidValue;
     const dim3 g(static_cast<uint32_t>(fu + mu)), b(256);
+    if (few.w.schedule || many.w.schedule)
+        hipLaunchKernelGGL(k_paged_schedule, dim3(2), dim3(1024), 0, s, a, few.w, many.w);
     if (many.used)
         hipLaunchKernelGGL((k_paged_chunks<T, HD, F32>), g, b, 0, s, a, many.w, few.w, static_cast<uint32_t>(mu));
     else
@@ -1065,13 +1174,14 @@ hipError_t attention_hd(const PagedAttentionArgs& a, const Half& few, const Half
 uint32_t paged_attention_launches(const PagedAttentionArgs& a) {
     Half few, many;
     halves(a, few, many);
-    return few.splits || many.splits ? 2u : 1u;
+    return (few.splits || many.splits ? 2u : 1u) + (a.requests > kWaveRequests ? 1u : 0u);
 }
 
 size_t paged_attention_work_floats(const PagedAttentionArgs& a) {
     Half few, many;
     halves(a, few, many);
-    return (few.part_floats() + many.part_floats()) * (a.kv.head_dim + 2u) + few.words() + many.words();
+    return (few.part_floats() + many.part_floats()) * (a.kv.head_dim + 2u) + few.words() + many.words() +
+           few.schedule_words(a.requests) + many.schedule_words(a.requests);
 }
 
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, float* work, hipStream_t s) {
@@ -1079,6 +1189,8 @@ hipError_t launch_paged_attention(const PagedAttentionArgs& a, float* work, hipS
     halves(a, few, many);
     float* at = work;
     for (Half* half : {&few, &many}) {
+        if (half->schedule_words(a.requests)) half->w.schedule = reinterpret_cast<uint32_t*>(at);
+        at += half->schedule_words(a.requests);
         if (!half->splits) continue;
         half->w.part = at;
         at += half->part_floats() * (a.kv.head_dim + 2u);

@@ -531,6 +531,19 @@ def test_attention_many_requests(hip, requests):
     check_attention(c, run_attention(hip, c))
 
 
+@pytest.mark.parametrize("requests", (64, 192, 193, 256, 1030, 4096, 4097, 8192))
+def test_attention_requests_beyond_a_wave(hip, requests):
+    """Where every wave finds its piece by itself and where a launch before leaves the sums:
+    rows long enough to be cut, requests without a row in between."""
+    g = np.random.default_rng(requests)
+    lens, new = P.ragged(g, requests, 90 if requests < 2000 else 12, 2)
+    lens[7], new[7] = 400, 70
+    lens[-1], new[-1], lens[-3], new[-3] = 6000, 1, 3000, 33
+    new[10:40] = [0] * 30
+    c = attention_case(requests, lens, new, 2, 1, 64, "F16", "F16", 8)
+    check_attention(c, run_attention(hip, c))
+
+
 def test_attention_order_does_not_change_bits(hip):
     c = attention_case(13, [3000, 700], [1, 1], 8, 2, 128, "F32", "F16", 16)
     first = run_attention(hip, c)
