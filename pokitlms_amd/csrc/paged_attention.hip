@@ -217,7 +217,9 @@ __device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, const Ro
     p.q0 = q.q0;
     p.fresh = q.q1 - q.q0;
     p.len = static_cast<int32_t>(q.len < positions ? q.len : positions);
-    return true;
+    // (sums of a query_start that decreases may leave their words and the scratch)
+    return left < q.work.tiles * p.parts &&
+           (p.parts == 1u || split_fits(p.split, p.slot, a.kv.kv_heads, 1u << w.log_target));
 }
 
 // What find_piece needs where there are more requests than lanes: a workgroup per kind of
@@ -958,13 +960,16 @@ struct SplitTile {
     uint64_t stride;  // floats from a part to the next
     const float* base;
 };
-// Entry i, if there is one (entries past the last hold what an earlier call left).
+// Entry i, if there is one (entries past the last hold what an earlier call left, and so do
+// those of tiles that no workgroup took, where query_start decreases).
 __device__ __forceinline__ bool split_tile(const PagedAttentionArgs& a, const RowWork& w, uint32_t bm, uint32_t i, SplitTile& t) {
     const u32x4* h = reinterpret_cast<const u32x4*>(w.head + kHeadWords * i);
     const uint32_t HD = a.kv.head_dim, hk = i % a.kv.kv_heads, count = w.count[0];
     const u32x4 x = h[0];
     const uint32_t slot = h[1][0];
-    if (i >= count) return false;
+    if (i >= count || !split_entry_fits(x[0], slot, x[1], x[2], x[3], a.group.by, bm, a.max_new, a.max_tokens,
+                                        a.kv.kv_heads, 1u << w.log_target))
+        return false;
     t.p = Piece{};
     t.parts = x[0];
     t.p.parts = 1u;

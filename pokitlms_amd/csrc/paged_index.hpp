@@ -116,4 +116,20 @@ PK_BOTH uint64_t most_units(uint64_t tiles, uint32_t kv_heads, uint32_t target) 
 // parts are fewer than 1.8 keys / pieces.
 PK_BOTH constexpr uint64_t most_parts(uint32_t target) { return 2ull * target; }
 
+// Whether a split tile's entry and the last of its parts, both counted per kv head, lie in
+// the scratch that these bounds give.  They always do where query_start does not decrease;
+// where it does, rows can be more than max_tokens and the bounds do not hold.
+PK_BOTH bool split_fits(uint32_t split, uint32_t last_part, uint32_t kv_heads, uint32_t target) {
+    return (split + 1ull) * kv_heads <= target && (last_part + 1ull) * kv_heads <= most_parts(target);
+}
+// Whether an entry of the split tiles' list, as read back, is one of this call's size.
+PK_BOTH bool split_entry_fits(uint32_t parts, uint32_t first_part, uint32_t q0, uint32_t fresh, uint32_t tile,
+                              uint32_t group, uint32_t bm, uint32_t max_new, uint32_t max_tokens, uint32_t kv_heads,
+                              uint32_t target) {
+    const uint64_t most = most_parts(target);
+    return parts > 1u && parts <= most && first_part < most && (0ull + first_part + parts) * kv_heads <= most &&
+           fresh && paged_new(q0, q0 + fresh, max_new, max_tokens) == fresh &&
+           static_cast<uint64_t>(tile) * bm < static_cast<uint64_t>(fresh) * group;
+}
+
 }  // namespace pk

@@ -110,6 +110,32 @@ void bad_lengths(uint32_t at) {
     CHECK(n <= most && (n == 0 || (q0 + n == q1 && q1 <= tokens)));
 }
 
+// What the kernels do with the sums and entries of any query_start, in their 32-bit words:
+// nothing that is taken lies outside the scratch or the rows.
+void broken_starts(uint32_t at) {
+    const uint32_t target = 1u << (9 + at % 2), kv_heads = 1 + draw(at % 3 ? 16 : 4096), group = 1 + draw(16);
+    const uint32_t bm = at % 2 ? 16 : 128, max_tokens = 1 + draw(5000), max_new = 1 + draw(max_tokens);
+    const uint32_t most = 2 * target;
+    for (int i = 0; i < 20; ++i) {
+        const uint32_t split = draw(i % 2 ? 2000 : 0xffffffffu), part = draw(i % 3 ? 4000 : 0xffffffffu);
+        if (pk::split_fits(split, part, kv_heads, target))
+            CHECK(uint64_t(split) * kv_heads + kv_heads <= target && uint64_t(part) * kv_heads + kv_heads <= most);
+        const bool any = i % 4 == 0;
+        const uint32_t parts = draw(any ? 0xffffffffu : 40), first = draw(any ? 0xffffffffu : 3000);
+        const uint32_t q0 = draw(any ? 0xffffffffu : 6000), fresh = draw(any ? 0xffffffffu : 6000);
+        const uint32_t tile = draw(any ? 0xffffffffu : 600);
+        if (pk::split_entry_fits(parts, first, q0, fresh, tile, group, bm, max_new, max_tokens, kv_heads, target)) {
+            CHECK(parts >= 2 && (uint64_t(first) + parts) * kv_heads <= most && uint64_t(q0) + fresh <= max_tokens);
+            CHECK(uint64_t(tile) * bm < uint64_t(fresh) * group);
+        }
+    }
+    // an entry that a call without a fault writes is taken
+    const uint32_t fresh = 1 + draw(max_new), q0 = draw(max_tokens - fresh + 1);
+    const uint32_t tile = draw((fresh * group + bm - 1) / bm), kvh = 1 + draw(target / 2);
+    CHECK(pk::split_entry_fits(2, most / kvh - 2, q0, fresh, tile, group, bm, max_new, max_tokens, kvh, target));
+    CHECK(pk::split_fits(target / kvh - 1, most / kvh - 1, kvh, target));
+}
+
 }  // namespace
 
 int main() {
@@ -118,6 +144,7 @@ int main() {
     for (; at < 60000; ++at) schedule(at);
     for (; at < 80000; ++at) bad_lengths(at);
     for (; at < 100000; ++at) divide(at);
+    for (; at < 130000; ++at) broken_starts(at);
     std::printf("ok %u\n", at);
     return 0;
 }

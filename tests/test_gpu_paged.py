@@ -544,6 +544,31 @@ def test_attention_requests_beyond_a_wave(hip, requests):
     check_attention(c, run_attention(hip, c))
 
 
+@pytest.mark.parametrize("requests", (6, 300))
+def test_attention_starts_that_decrease(hip, requests):
+    """A query_start that decreases: more rows than max_tokens, so that not all of the work
+    has a workgroup.  What the rows get is not said; nothing beyond max_tokens is written,
+    and the next call is right."""
+    c = attention_case(20, [6000] * requests if requests < 10 else [700] * requests, [6] * requests, 4, 2, 64, "F16",
+                       "F16", 64)
+    rows = 30
+    assert rows < c["q"].shape[0]
+    for start in ([0] + [rows, 3] * (requests // 2), [0, 25] * (requests // 2) + [7],
+                  [rows - 1, rows] * (requests // 2) + [2]):
+        out = torch.full_like(c["q"], 5.0)
+        hip.paged_attention_async(attention_call(dict(c, start=np.array(start), rows=rows), out))
+        torch.cuda.synchronize()
+        assert torch.all(out[rows:] == 5.0)
+    check_attention(c, run_attention(hip, c))
+
+
+@pytest.mark.parametrize("gtype,cache", TYPES)
+def test_attention_smallest_scale(hip, gtype, cache):
+    """The smallest positive scale: all scores are alike, masked ones still have no weight."""
+    c = attention_case(21, [5, 70, 300], [5, 40, 1], 4, 2, 64, gtype, cache, 16)
+    check_attention(c, run_attention(hip, c, scale=1e-45), scale=1e-45)
+
+
 def test_attention_order_does_not_change_bits(hip):
     c = attention_case(13, [3000, 700], [1, 1], 8, 2, 128, "F32", "F16", 16)
     first = run_attention(hip, c)
