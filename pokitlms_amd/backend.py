@@ -18,6 +18,7 @@ kernels of ``csrc/``.
 from __future__ import annotations
 
 import ctypes
+import threading
 from dataclasses import dataclass
 
 import numpy as np
@@ -132,6 +133,13 @@ class Moe35LayerHandles(MoeLayerHandles):
             w.release()
 
 
+class _ErrorText(threading.local):
+    """A thread's buffer for the text of a refusal."""
+
+    def __init__(self):
+        self.buffer = ctypes.create_string_buffer(_ERRBUF)
+
+
 class PagedKV:
     """One layer's paged KV cache in device memory the caller owns (pk_hip_paged_kv):
     k and v addresses, GGUF type (F16 or BF16), strides in elements (all 0: rows
@@ -229,7 +237,7 @@ class HipBackend:
         self.handle = h.value
         self._cache = {}
         # the paged calls come many times a step: their functions and error text are kept
-        self._err = ctypes.create_string_buffer(_ERRBUF)
+        self._text = _ErrorText()
         self._plan, self._append = L.pk_hip_paged_plan_async, L.pk_hip_paged_append_async
         self._attend = L.pk_hip_paged_attention_async
 
@@ -587,21 +595,24 @@ class HipBackend:
     # ---- paged KV cache ---------------------------------------------------------------
     def paged_plan_async(self, plan: PagedPlan, stream: int = 0) -> None:
         """Pages, positions and slots of a step's new tokens (pk_hip_paged_plan_async)."""
-        status = self._plan(self.handle, plan.ref, stream or None, self._err, _ERRBUF)
+        err = self._text.buffer
+        status = self._plan(self.handle, plan.ref, stream or None, err, _ERRBUF)
         if status:
-            _raise(status, self._err)
+            _raise(status, err)
 
     def paged_append_async(self, append: PagedAppend, stream: int = 0) -> None:
         """Head norms, rotation and K and V into the pages (pk_hip_paged_append_async)."""
-        status = self._append(self.handle, append.ref, stream or None, self._err, _ERRBUF)
+        err = self._text.buffer
+        status = self._append(self.handle, append.ref, stream or None, err, _ERRBUF)
         if status:
-            _raise(status, self._err)
+            _raise(status, err)
 
     def paged_attention_async(self, attention: PagedAttention, stream: int = 0) -> None:
         """Attention of new tokens over the pages (pk_hip_paged_attention_async)."""
-        status = self._attend(self.handle, attention.ref, stream or None, self._err, _ERRBUF)
+        err = self._text.buffer
+        status = self._attend(self.handle, attention.ref, stream or None, err, _ERRBUF)
         if status:
-            _raise(status, self._err)
+            _raise(status, err)
 
     def sync(self, stream: int = 0) -> None:
         err = ctypes.create_string_buffer(_ERRBUF)

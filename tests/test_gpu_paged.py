@@ -1,4 +1,6 @@
 """The paged-cache operators on the GPU against plain 64-bit numpy (tests/paged.py)."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -789,3 +791,28 @@ def test_calls_are_counted_and_timed(hip):
     after = hip.stats()
     assert after["paged_attention_calls"] == before["paged_attention_calls"] + 1
     assert after["paged_attention_ns"] > before["paged_attention_ns"]
+
+
+def test_refusals_of_two_threads_keep_their_texts(hip):
+    """Calls of two threads at once: each raises its own refusal."""
+    kv = PagedKV(1 << 20, 1 << 20, 1, 4, 16, 1, 64)
+    calls = {"out may not be q": PagedAttention(kv, 1, 1, 1, 1, q=4096, out=4096, query_start=64, lens=64,
+                                                block_table=64, table_stride=1),
+             "requests must be between": PagedAttention(kv, 1, 1, 0, 1, q=4096, out=8192, query_start=64, lens=64,
+                                                        block_table=64, table_stride=1)}
+    wrong = []
+
+    def run(text):
+        for _ in range(2000):
+            try:
+                hip.paged_attention_async(calls[text])
+                wrong.append("no refusal")
+            except ValueError as e:
+                if text not in str(e):
+                    wrong.append(str(e))
+    threads = [threading.Thread(target=run, args=(text,)) for text in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
