@@ -616,8 +616,9 @@ pk_hip_status pk_hip_paged_append_async(pk_hip_ctx* ctx, const pk_hip_paged_appe
 
 /* Causal attention of new tokens: rows query_start[r] .. query_start[r + 1] - 1 of q
  * are the last positions of request r, whose lens[r] positions (these included) lie in
- * its pages (a length past what a row of the table holds counts as that).  The row of position p sees position i if i <= p, i's page is there, and,
- * with a window, i + window > p or i < sinks:
+ * its pages (a length past what a row of the table holds counts as that).  The row of
+ * position p sees position i if i <= p, i's page is there, and, with a window, i + window
+ * > p or i < sinks:
  *   out = sum_i softmax_i(scale * q . k_i) v_i (KvCache::attend, src/kv_cache.cpp:
  * 219-294), head h over kv head h / (heads / kv_heads), and 0 where nothing is seen.
  * Decoding requests, chunks of prompts and requests without a row mix freely.  q and out
