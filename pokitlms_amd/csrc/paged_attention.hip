@@ -467,8 +467,10 @@ __device__ __forceinline__ void load_q(const PagedAttentionArgs& a, uint64_t at,
 // (l % 16) * HD / 16 + e is row l % 16 of product e.  Reading K and V bounds it: the next
 // K is on its way while the weights are taken, the next V while the next scores are.  32
 // heads over 4 of 128, F16: 131,072 positions 42.5 us (6.3 TB/s); 64 requests up to 8192
-// positions, BF16, 70 us (4.8 TB/s, uneven requests); eight of 512, F32, 10.4 us, where a
-// workgroup's 128 keys cost 1.3 us, one latency of memory.
+// positions, BF16, 70 us (4.8 TB/s, uneven requests); eight of 512, F32, 10.4 us, where the
+// 64 KB of a workgroup's 128 keys take a CU 1.3 us (50 GB/s).  Eight waves share out the same
+// reading: eight requests of 500 10.2 -> 10.0 us, one of 131,072 57.9 -> 56.6, 64 up to 8192
+// 79 -> 89.
 template <uint32_t HD>
 struct RowsLds {
     alignas(16) uint64_t off[4][32];
