@@ -1120,30 +1120,34 @@ struct Half {
     uint32_t bm;
     bool used, splits;
     uint64_t tiles;  // at most, over all kv heads
+    uint32_t keys;   // pieces that a tile sees at most
     uint32_t target() const { return 1u << w.log_target; }
     uint64_t part_floats() const { return splits ? most_parts(target()) * bm : 0u; }
     uint64_t words() const { return splits ? target() * kHeadWords + 4u : 0u; }  // a split tile has two parts
     uint32_t schedule_words(uint32_t requests) const {
         return used && requests > kWaveRequests ? (pk::schedule_words(requests) + 3u) / 4u * 4u : 0u;
     }
-    uint64_t units(uint32_t kv_heads) const { return most_units(tiles / kv_heads, kv_heads, splits ? target() : 0u) * kv_heads; }
+    uint64_t units(uint32_t kv_heads) const {
+        return (splits ? most_units_seen(tiles / kv_heads, kv_heads, target(), keys, w.least) : tiles / kv_heads) * kv_heads;
+    }
     uint32_t split_tiles() const { return !splits ? 0u : tiles < target() ? static_cast<uint32_t>(tiles) : target(); }
 };
 void halves(const PagedAttentionArgs& a, Half& few, Half& many) {
     const uint64_t positions = static_cast<uint64_t>(a.table_stride) << a.kv.page_shift;
-    const bool may_split = positions / kScheduleKeys + 2u > kLeast + kLeast / 4u;
     const uint32_t group = a.group.by;
     // a request of the 16-row tiles has at most kFewRows rows
     const uint64_t n = a.requests < a.max_tokens ? a.requests : a.max_tokens;
     const uint64_t tokens = n * (kFewRows / group ? kFewRows / group : 1u);
     few = Half{{1u, kFewRows, kRowsTarget, kLeast, nullptr, nullptr, nullptr, nullptr}, 16u, group <= kFewRows, false,
-               most_tiles(tokens < a.max_tokens ? tokens : a.max_tokens, a.requests, group, 16u) * a.kv.kv_heads};
+               most_tiles(tokens < a.max_tokens ? tokens : a.max_tokens, a.requests, group, 16u) * a.kv.kv_heads,
+               most_keys(a.group, 16u, a.window, a.sinks, positions)};
     if (few.tiles < kFewTiles) few.w.log_target = kFewTilesTarget;
     many = Half{{kFewRows + 1u, 0xffffffffu, kTilesTarget, kLeast, nullptr, nullptr, nullptr, nullptr}, kTileRows,
                 static_cast<uint64_t>(a.max_new) * group > kFewRows, false,
-                most_tiles(a.max_tokens, a.requests, group, kTileRows) * a.kv.kv_heads};
-    few.splits = may_split && few.used;
-    many.splits = may_split && many.used;
+                most_tiles(a.max_tokens, a.requests, group, kTileRows) * a.kv.kv_heads,
+                most_keys(a.group, kTileRows, a.window, a.sinks, positions)};
+    few.splits = few.used && request_parts(few.keys, kLeast) > 1u;
+    many.splits = many.used && request_parts(many.keys, kLeast) > 1u;
 }
 
 template <uint32_t T, uint32_t HD, bool F32>

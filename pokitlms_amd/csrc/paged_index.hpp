@@ -112,6 +112,19 @@ PK_BOTH uint64_t most_tiles(uint64_t max_tokens, uint64_t requests, uint64_t gro
 PK_BOTH uint64_t most_units(uint64_t tiles, uint32_t kv_heads, uint32_t target) {
     return tiles + (target + kv_heads - 1u) / kv_heads;
 }
+// Pieces that a row tile sees at most: those of a table row, or of a window, the tile's own
+// tokens and the sinks.
+PK_BOTH uint32_t most_keys(const Divide& group, uint32_t bm, uint32_t window, uint32_t sinks, uint64_t positions) {
+    const uint64_t all = (positions + kScheduleKeys - 1u) / kScheduleKeys;
+    const uint64_t seen = (static_cast<uint64_t>(window) + group(bm) + 1u) / kScheduleKeys + 2u +
+                          (static_cast<uint64_t>(sinks) + kScheduleKeys - 1u) / kScheduleKeys;
+    return static_cast<uint32_t>(window && seen < all ? seen : all);
+}
+// Workgroups per kv head where a tile sees at most `keys` pieces: its parts are then few.
+PK_BOTH uint64_t most_units_seen(uint64_t tiles, uint32_t kv_heads, uint32_t target, uint32_t keys, uint32_t least) {
+    const uint64_t a = most_units(tiles, kv_heads, target), b = tiles * ((keys + least - 1u) / least);
+    return b < a ? b : a;
+}
 // Parts of split tiles, over all kv heads: a split tile sees more than 1.25 pieces, so its
 // parts are fewer than 1.8 keys / pieces.
 PK_BOTH constexpr uint64_t most_parts(uint32_t target) { return 2ull * target; }

@@ -96,6 +96,35 @@ void schedule(uint32_t at) {
     if (positions / pk::kScheduleKeys + 2 <= least + least / 4) CHECK(parts == 0);
 }
 
+// Tiles of any length see no more pieces than most_keys says, with that the workgroups
+// suffice, and a call without a tile that could be cut has none that is.
+void windows(uint32_t at) {
+    const uint32_t bm = draw(2) ? 16 : 128, group = 1 + draw(draw(2) ? 9 : 200), kv_heads = 1 + draw(8);
+    const uint32_t log_target = 3 + draw(8), target = 1u << log_target, least = 1 + draw(9), requests = 1 + draw(30);
+    const uint32_t window = draw(4) ? 1 + draw(draw(2) ? 3000 : 200) : 0, sinks = draw(3) ? draw(300) : 0;
+    const uint32_t positions = 1 + draw(draw(2) ? 20000 : 900);
+    const pk::Divide by = pk::divide_by(group);
+    const uint32_t most = pk::most_keys(by, bm, window, sinks, positions);
+    uint64_t work = 0, tiles = 0, units = 0, split = 0;
+    std::vector<pk::RequestWork> all;
+    for (uint32_t r = 0; r < requests; ++r) {
+        const uint32_t fresh = draw(3) ? 1 + draw(3) : 1 + draw(700);
+        const uint32_t len = draw(4) ? draw(positions + 1) : fresh + draw(positions);
+        all.push_back(pk::request_work(fresh, len, by, bm, 1, 0xffffffffu, window, sinks, positions));
+        CHECK(all[r].keys <= most);
+        work += uint64_t(all[r].tiles) * all[r].keys;
+        tiles += all[r].tiles;
+    }
+    const uint32_t pieces = pk::part_pieces(work * kv_heads, log_target, least);
+    for (const pk::RequestWork& r : all) {
+        const uint32_t n = pk::request_parts(r.keys, pieces);
+        units += uint64_t(r.tiles) * n;
+        split += n > 1 ? r.tiles : 0;
+    }
+    if (pk::request_parts(most, least) == 1) CHECK(split == 0 && units == tiles);
+    else CHECK(units <= pk::most_units_seen(tiles, kv_heads, target, most, least));
+}
+
 void divide(uint32_t at) {
     const uint32_t d = 1 + draw(at % 2 ? 40 : 5000);
     const pk::Divide by = pk::divide_by(d);
@@ -145,6 +174,7 @@ int main() {
     for (; at < 80000; ++at) bad_lengths(at);
     for (; at < 100000; ++at) divide(at);
     for (; at < 130000; ++at) broken_starts(at);
+    for (; at < 190000; ++at) windows(at);
     std::printf("ok %u\n", at);
     return 0;
 }
