@@ -931,9 +931,14 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
     }
 }
 
+// At most 256 registers up to head_dim 128 (two workgroups a CU): given 512, the compiler keeps
+// operands in the accumulator half and moves them over for every tile.  F32 rows, four chunks
+// of 512 over 2048, 16 heads over 4: of 128 over F16 118 us, with 256 88, over BF16 135 and 110
+// (a few spills), of 64 over F16 65 and 59.  At 256 the LDS holds one workgroup; its single
+// tokens, held to 256 registers, would spill (16 of 2000, F32: 30 us, 57).
 // One launch: the tiles' workgroups first, they take longest.
 template <uint32_t T, uint32_t HD, bool F32>
-__global__ __launch_bounds__(256, HD <= 128u && !F32 ? 2 : 1) void k_paged_chunks(PagedAttentionArgs a, RowWork many,
+__global__ __launch_bounds__(256, HD <= 128u ? 2 : 1) void k_paged_chunks(PagedAttentionArgs a, RowWork many,
                                                                                 RowWork few, uint32_t tile_blocks) {
     __shared__ union Lds {
         TilesLds<HD> tiles;
@@ -944,7 +949,7 @@ __global__ __launch_bounds__(256, HD <= 128u && !F32 ? 2 : 1) void k_paged_chunk
 }
 
 template <uint32_t T, uint32_t HD, bool F32>
-__global__ __launch_bounds__(256) void k_paged_rows(PagedAttentionArgs a, RowWork few) {
+__global__ __launch_bounds__(256, HD <= 128u ? 2 : 1) void k_paged_rows(PagedAttentionArgs a, RowWork few) {
     __shared__ RowsLds<HD> lds;
     rows_piece<T, HD, F32>(a, few, blockIdx.x, lds);
 }
