@@ -863,7 +863,8 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
         __builtin_amdgcn_sched_group_barrier(0x008, 6u * NP, 0);
         const bool cut = there != ~0ull || static_cast<int32_t>(base + KT) - 1 > w_first ||
                          (a.window && base + a.window <= static_cast<uint32_t>(w_last) && base + KT > a.sinks);
-        const bool watch = cut && w_first != w_last && !any_nan(o);
+        // (what is loaded of V goes by the whole tile's rows, also where this wave's stand at one position)
+        const bool watch = cut && p_first != p_last && !any_nan(o);
         if (cut) {
             const uint64_t mine = there >> (4u * h);
 #pragma unroll
@@ -910,7 +911,7 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
                     for (uint32_t i = 0; i < NP; ++i) o[d] = M::mma32(__builtin_bit_cast(V8, x), pp[i], o[d]);
                 }
             }
-        if (cut && w_first != w_last) suspect = suspect || (watch && any_nan(o));
+        if (cut && p_first != p_last) suspect = suspect || (watch && any_nan(o));
     }
     if (!wave_live) return;
     l += __shfl_xor(l, 32u);
