@@ -342,10 +342,65 @@ __device__ __forceinline__ bool any_nan(const V (&o)[N]) {
     return nan;
 }
 
-// One row over the key tiles t0 .. t1 - 1 by one wave, reading only what the row sees: for
-// rows into which a masked value (NaN or infinite, with weight 0) may have come by way of a
-// tile whose other rows see it, that is, whose sums turned NaN in a tile of which they see
-// a part.
+// V is loaded for all rows of a tile, so a row that does not see a NaN or an infinity there takes
+// it with weight 0, which makes NaN.  Rows whose sums are NaN in the end are rare; then one more
+// look at V finds the positions that hold such values, and the rows that do not see all of
+// them are done again by themselves.  (Sums that are NaN because of what a row does see are
+// right, and cost that look alone.)
+constexpr uint32_t kNoPosition = 0x7fffffffu;
+struct OddValues {
+    uint32_t first, end;  // the first position a window can hide (or kNoPosition), the last one's + 1 (or 0)
+};
+// Of the key tiles t, t + step, .. below t1, loaded from lo on and for sinks up to p_last.
+__device__ OddValues odd_values(const PagedAttentionArgs& a, const Piece& p, const KeyTiles& keys, uint32_t kt,
+                                uint32_t t, uint32_t t1, uint32_t step, uint32_t hk, uint32_t lo, int32_t p_last) {
+    constexpr uint32_t U = 8u;
+    const uint32_t lane = threadIdx.x & 63u, lanes = a.kv.head_dim / 8u, rows = 64u / lanes;
+    const uint32_t positions = a.table_stride << a.kv.page_shift, mask = (1u << a.kv.page_shift) - 1u;
+    const uint32_t infinity = a.kv.type == T_F16 ? 0x7c00u : 0x7f80u;
+    const uint32_t* table = a.table + static_cast<uint64_t>(p.r) * a.table_stride;
+    OddValues odd{kNoPosition, 0u};
+    for (; t < t1; t += step) {
+        const uint32_t base = keys.base(t, kt), at = base + lane;
+        const bool in = lane < kt && static_cast<int32_t>(at) <= p_last && at < positions && (at >= lo || at < a.sinks);
+        const uint32_t page = in ? table[at >> a.kv.page_shift] : kNoSlot;
+        for (uint32_t r0 = lane / lanes; r0 < kt; r0 += U * rows) {
+            u32x4 x[U];
+            bool there[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t r = r0 + u * rows, pg = __shfl(page, r & 63u);
+                there[u] = r < kt && pg < a.kv.pages;
+                const uint64_t row = pg * a.kv.page_stride + ((base + r) & mask) * a.kv.slot_stride + hk * a.kv.head_stride;
+                x[u] = *reinterpret_cast<const u32x4*>(a.kv.v + (there[u] ? row + 8u * (lane % lanes) : 0u));
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                bool bad = false;
+#pragma unroll
+                for (uint32_t d = 0; d < 4; ++d)
+                    bad = bad || (x[u][d] & 0x7fffu) >= infinity || ((x[u][d] >> 16) & 0x7fffu) >= infinity;
+                const uint32_t i = base + r0 + u * rows;
+                if (bad && there[u]) {
+                    odd.end = odd.end > i ? odd.end : i + 1u;
+                    if (i >= a.sinks && i < odd.first) odd.first = i;
+                }
+            }
+        }
+    }
+    return odd;
+}
+// Of the rows f0 + i whose bit i of `nan` is set, those that do not see all odd positions.
+__device__ __forceinline__ uint32_t rows_again(const PagedAttentionArgs& a, const Piece& p, uint32_t f0, uint32_t nan,
+                                               const OddValues& odd) {
+    const uint32_t i = threadIdx.x & 31u;
+    const int32_t pos = p.len - static_cast<int32_t>(p.fresh) + static_cast<int32_t>(a.group(f0 + i));
+    const bool hidden = static_cast<int32_t>(odd.end) > pos + 1 ||
+                        (a.window && odd.first + a.window <= static_cast<uint32_t>(pos));
+    return static_cast<uint32_t>(__ballot(((nan >> i) & 1u) && hidden));
+}
+
+// One row over the key tiles t0 .. t1 - 1 by one wave, reading only what the row sees.
 __device__ void row_alone(const PagedAttentionArgs& a, const Piece& p, const KeyTiles& keys, uint32_t kt, uint32_t t0,
                           uint32_t t1, uint32_t hk, uint32_t f, const RowTo& to) {
     const uint32_t lane = threadIdx.x & 63u, HD = a.kv.head_dim, token = p.q0 + a.group(f);
@@ -476,7 +531,7 @@ struct RowsLds {
     alignas(16) uint64_t off[4][32];
     alignas(16) float o[4][16][HD + 4u];
     float m[4][16], l[4][16];
-    uint32_t bad;
+    uint32_t nan, first, end;
 };
 
 template <uint32_t T, uint32_t HD, bool F32>
@@ -493,7 +548,8 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
     if (!live_piece) return;
     if (tid == 0u) {
         write_head(a, w, p, hk);
-        lds.bad = 0u;
+        lds.nan = lds.end = 0u;
+        lds.first = kNoPosition;
     }
     const uint32_t rows = p.fresh * a.group.by - p.tile * BM < BM ? p.fresh * a.group.by - p.tile * BM : BM;
     const uint32_t positions = a.table_stride << a.kv.page_shift, mask = (1u << a.kv.page_shift) - 1u;
@@ -563,7 +619,6 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
 #pragma unroll
     for (uint32_t e = 0; e < DPL; ++e) o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
-    bool suspect = false;
     uint32_t b = b0 + wave, next_page = kNoSlot;
     if (b < b1) {
         place(b, entry(b));
@@ -592,7 +647,6 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
         // every row sees the whole tile, or each score asks
         const bool cut = here != 0xffffffffu || static_cast<int32_t>(base + KT) - 1 > p_first ||
                          (a.window && base + a.window <= static_cast<uint32_t>(p_last) && base + KT > a.sinks);
-        const bool watch = cut && p_first != p_last && !any_nan(o);
         if (cut) {
 #pragma unroll
             for (uint32_t t = 0; t < 2; ++t)
@@ -639,7 +693,6 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
         }
         if (more) load_v();
         __builtin_amdgcn_sched_barrier(0);
-        if (cut && p_first != p_last) suspect = suspect || (watch && any_nan(o));
     }
     // the four waves' parts
     l += __shfl_xor(l, 16u);
@@ -648,8 +701,8 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
         lds.m[wave][j] = m;
         lds.l[wave][j] = l;
     }
-    __syncthreads();  // lds.bad is 0 as well
-    if (suspect && j < rows && l == l) atomicOr(&lds.bad, 1u << j);
+    __syncthreads();  // lds.nan is 0 as well
+    if (j < rows && l == l && any_nan(o)) atomicOr(&lds.nan, 1u << j);
     {
         const float mm = fmaxf(fmaxf(lds.m[0][j], lds.m[1][j]), fmaxf(lds.m[2][j], lds.m[3][j]));
         const float keep = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mm);
@@ -666,7 +719,14 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
     float sum = 0.0f;
 #pragma unroll
     for (uint32_t v = 0; v < 4; ++v) sum += mm == -INFINITY ? lds.l[v][row] : lds.l[v][row] * __builtin_amdgcn_exp2f(lds.m[v][row] - mm);
-    const uint32_t again = lds.bad;
+    uint32_t again = lds.nan;
+    if (again) {
+        const OddValues odd = odd_values(a, p, keys, KT, b0 + wave, b1, 4u, hk, lo, p_last);
+        atomicMax(&lds.end, odd.end);
+        atomicMin(&lds.first, odd.first);
+        __syncthreads();
+        again = rows_again(a, p, p.tile * BM, again, {lds.first, lds.end});
+    }
     if (row < rows && !((again >> row) & 1u)) {
         const RowTo to = row_to(a, w, p, BM, hk, row);
 #pragma unroll
@@ -721,6 +781,7 @@ __device__ __forceinline__ void load_to_lds(const void* src, uint32_t offset, ui
 template <uint32_t HD>
 struct TilesLds {
     alignas(1024) uint8_t k[2][kTileKeys * 2u * HD], v[2][kTileKeys * 2u * HD];
+    uint32_t nan, first, end;
 };
 
 template <uint32_t T, uint32_t HD, bool F32>
@@ -736,7 +797,11 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
     const bool live_piece = find_piece(a, w, BM, block / a.kv.kv_heads, p, splits);
     if (w.count && block == 0u && tid == 0u) w.count[0] = splits * a.kv.kv_heads;
     if (!live_piece) return;
-    if (tid == 0u) write_head(a, w, p, hk);
+    if (tid == 0u) {
+        write_head(a, w, p, hk);
+        lds.nan = lds.end = 0u;
+        lds.first = kNoPosition;
+    }
     const uint32_t left = p.fresh * a.group.by - p.tile * BM, rows = left < BM ? left : BM;
     const uint32_t positions = a.table_stride << a.kv.page_shift, mask = (1u << a.kv.page_shift) - 1u;
     const int32_t p0 = p.len - static_cast<int32_t>(p.fresh);
@@ -819,7 +884,6 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
 #pragma unroll
         for (uint32_t x = 0; x < 16; ++x) o[d][x] = 0.0f;
     float m = -INFINITY, l = 0.0f;
-    bool suspect = false;
     uint64_t next_there = 0;
     uint32_t page = kNoSlot;
     if (t0 < t1) {
@@ -863,8 +927,6 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
         __builtin_amdgcn_sched_group_barrier(0x008, 6u * NP, 0);
         const bool cut = there != ~0ull || static_cast<int32_t>(base + KT) - 1 > w_first ||
                          (a.window && base + a.window <= static_cast<uint32_t>(w_last) && base + KT > a.sinks);
-        // (what is loaded of V goes by the whole tile's rows, also where this wave's stand at one position)
-        const bool watch = cut && p_first != p_last && !any_nan(o);
         if (cut) {
             const uint64_t mine = there >> (4u * h);
 #pragma unroll
@@ -911,13 +973,12 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
                     for (uint32_t i = 0; i < NP; ++i) o[d] = M::mma32(__builtin_bit_cast(V8, x), pp[i], o[d]);
                 }
             }
-        if (cut && p_first != p_last) suspect = suspect || (watch && any_nan(o));
     }
-    if (!wave_live) return;
     l += __shfl_xor(l, 32u);
-    uint64_t again = __ballot(suspect && live && l == l);
-    again = (again | (again >> 32)) & 0xffffffffu;
-    if (live && !((again >> j) & 1u)) {
+    const uint64_t either = __ballot(live && l == l && any_nan(o));
+    const uint32_t nan = static_cast<uint32_t>(either | (either >> 32));
+    if (nan && lane == 0u) atomicOr(&lds.nan, 1u);  // (a barrier of the loop ago it was set to 0)
+    if (live) {
         const RowTo to = row_to(a, w, p, BM, hk, 32u * wave + j);
 #pragma unroll
         for (uint32_t d = 0; d < DT; ++d)
@@ -925,8 +986,16 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
             for (uint32_t x = 0; x < 16; x += 4)
                 store_row4(a, to, 32u * d + 2u * x + 4u * h, f32x4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]}, m, l);
     }
+    __syncthreads();
+    if (!lds.nan) return;
+    const OddValues odd = odd_values(a, p, keys, KT, t0 + wave, t1, 4u, hk, lo, p_last);
+    atomicMax(&lds.end, odd.end);
+    atomicMin(&lds.first, odd.first);
+    __syncthreads();
+    // (the stores of the rows that are done again came before the barrier)
+    uint32_t again = rows_again(a, p, f0, nan, {lds.first, lds.end});
     while (again) {
-        const uint32_t i = static_cast<uint32_t>(__builtin_ctzll(again));
+        const uint32_t i = static_cast<uint32_t>(__builtin_ctz(again));
         again &= again - 1u;
         row_alone(a, p, keys, KT, t0, t1, hk, f0 + i, row_to(a, w, p, BM, hk, 32u * wave + i));
     }

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from tests import paged as P
-from tests.test_gpu_paged import attention_case, f64, run_attention
+from tests.test_gpu_paged import TYPES, attention_call, attention_case, f64, run_attention
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -27,7 +27,7 @@ def close(c, got, rows, window=0, sinks=0, columns=slice(None)):
     ref = clean(c)
     want, bound = P.attention(f64(ref["q"]), f64(ref["k"]), f64(ref["v"]), c["table"], c["start"], c["lens"], c["page"],
                               c["dim"] ** -0.5, window, sinks)
-    tol = P.attention_tolerance(np.nan_to_num(want), bound, c["dim"], c["gtype"], c["cache"])
+    tol = np.broadcast_to(P.attention_tolerance(np.nan_to_num(want), bound, c["dim"], c["gtype"], c["cache"]), want.shape)
     got = f64(got)[rows][..., columns]
     assert np.all(np.isfinite(got))
     assert np.all(np.abs(got - want[rows][..., columns]) <= tol[rows][..., columns])
@@ -57,3 +57,53 @@ def test_hidden_by_a_window_beside_rows_of_one_position(hip, gtype, cache, heads
     got = run_attention(hip, c, window=50)
     close(c, got, [new - 1], window=50)
     assert not torch.isfinite(got[0].float()).any()  # and the first row does see it
+
+
+@pytest.mark.parametrize("gtype,cache", TYPES)
+@pytest.mark.parametrize("new", (3, 40))
+@pytest.mark.parametrize("bad", (NAN, INF))
+def test_a_seen_nan_does_not_hide_a_masked_one(hip, gtype, cache, new, bad):
+    """Rows that see a NaN in one column keep the masked values of a later token out of the
+    others."""
+    c = attention_case(72, [160], [new], 4, 2, 128, gtype, cache, 16)
+    c["v"][slot(c, 0, 3)][0, 5] = NAN
+    c["v"][slot(c, 0, 159)][:, 6] = bad
+    got = run_attention(hip, c)
+    rest = [i for i in range(128) if i != 5]
+    rows = list(range(new - 1))
+    close(c, got, rows, columns=rest)
+    assert torch.isnan(got[:new, :2, 5]).all()
+    assert torch.isfinite(got[rows, 2:, 5].float()).all()
+
+
+# ---- what a NaN that rows see costs ---------------------------------------------------
+
+def least_time(hip, c):
+    """Of several calls, the shortest time between events around it, in ms."""
+    out = torch.full_like(c["q"], 5.0)
+    call, best = attention_call(c, out), INF
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(8):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record(stream)
+        hip.paged_attention_async(call, stream.cuda_stream)
+        b.record(stream)
+        stream.synchronize()
+        if i:
+            best = min(best, a.elapsed_time(b))
+    return best
+
+
+@pytest.mark.parametrize("gtype,cache", [("BF16", "BF16"), ("F32", "F16")])
+def test_seen_nan_does_not_do_rows_again(hip, gtype, cache):
+    """Rows that see a NaN, in one column or all, are not done again by themselves: another look
+    at their keys and values, no more."""
+    c = attention_case(78, [4000], [4000], 8, 2, 128, gtype, cache, 16)
+    plain = least_time(hip, c)
+    for name, column in (("v", 5), ("k", 5), ("v", slice(None))):
+        bad = {**c, name: c[name].clone()}
+        bad[name][slot(c, 0, 64)][:, column] = NAN
+        spent = least_time(hip, bad)
+        print(f"{gtype} {name} {column}: {plain:.3f} -> {spent:.3f} ms")
+        assert spent < 6 * plain
