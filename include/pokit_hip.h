@@ -626,7 +626,8 @@ pk_hip_status pk_hip_paged_append_async(pk_hip_ctx* ctx, const pk_hip_paged_appe
  * (F32: q and the weights enter the products as two or three parts, else the weights are
  * rounded to the cache's type).  Requests with more than max_new rows, and rows of no
  * request, are left as they were.  What masked positions hold, NaN too, does not
- * matter. */
+ * matter; infinities that a row sees count as the formula says in FP32, and a row of
+ * which every score is -inf as one that sees nothing. */
 typedef struct pk_hip_paged_attention {
     pk_hip_paged_kv cache;
     uint32_t type;               /* of q and out */

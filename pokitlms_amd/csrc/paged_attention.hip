@@ -342,30 +342,36 @@ __device__ __forceinline__ bool any_nan(const V (&o)[N]) {
     return nan;
 }
 
-// V is loaded for all rows of a tile, so a row that does not see a NaN or an infinity there takes
-// it with weight 0, which makes NaN.  Rows whose sums are NaN in the end are rare; then one more
-// look at V finds the positions that hold such values, and the rows that do not see all of
-// them are done again by themselves.  (Sums that are NaN because of what a row does see are
-// right, and cost that look alone.)
+// Where the products make NaN and the definition does not.  V is loaded for all rows of a tile, so
+// a row that does not see a NaN or an infinity there takes it with weight 0.  And a part of
+// q or of a weight can be 0, or of the other sign than the whole: an infinity that a row does
+// see, times the parts, is NaN where the score is -inf or the output infinite.  (So can a
+// weight that its type rounds to 0.)  Rows whose sums are NaN in the end are rare; then one
+// more look at V, for F32 rows at K too, finds the positions that hold NaN or infinities, and
+// the rows that do not see all of them, or all if there is an infinity, are done again by
+// themselves.  Sums that are NaN because of a NaN that a row sees are right, and cost that look.
 constexpr uint32_t kNoPosition = 0x7fffffffu;
 struct OddValues {
-    uint32_t first, end;  // the first position a window can hide (or kNoPosition), the last one's + 1 (or 0)
+    uint32_t first, end;  // V's first position that a window can hide (or kNoPosition), its last one's + 1 (or 0)
+    uint32_t infinite;    // whether there is an infinity
 };
 // Of the key tiles t, t + step, .. below t1, loaded from lo on and for sinks up to p_last.
-__device__ OddValues odd_values(const PagedAttentionArgs& a, const Piece& p, const KeyTiles& keys, uint32_t kt,
-                                uint32_t t, uint32_t t1, uint32_t step, uint32_t hk, uint32_t lo, int32_t p_last) {
+__device__ __forceinline__ OddValues odd_values(const PagedAttentionArgs& a, const Piece& p, const KeyTiles& keys,
+                                                uint32_t kt, uint32_t t, uint32_t t1, uint32_t step, uint32_t hk,
+                                                uint32_t lo, int32_t p_last) {
     constexpr uint32_t U = 8u;
     const uint32_t lane = threadIdx.x & 63u, lanes = a.kv.head_dim / 8u, rows = 64u / lanes;
     const uint32_t positions = a.table_stride << a.kv.page_shift, mask = (1u << a.kv.page_shift) - 1u;
     const uint32_t infinity = a.kv.type == T_F16 ? 0x7c00u : 0x7f80u;
     const uint32_t* table = a.table + static_cast<uint64_t>(p.r) * a.table_stride;
-    OddValues odd{kNoPosition, 0u};
+    const bool f32 = a.type == T_F32;
+    OddValues odd{kNoPosition, 0u, 0u};
     for (; t < t1; t += step) {
         const uint32_t base = keys.base(t, kt), at = base + lane;
         const bool in = lane < kt && static_cast<int32_t>(at) <= p_last && at < positions && (at >= lo || at < a.sinks);
         const uint32_t page = in ? table[at >> a.kv.page_shift] : kNoSlot;
         for (uint32_t r0 = lane / lanes; r0 < kt; r0 += U * rows) {
-            u32x4 x[U];
+            u32x4 x[U], y[U];
             bool there[U];
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u) {
@@ -373,13 +379,20 @@ __device__ OddValues odd_values(const PagedAttentionArgs& a, const Piece& p, con
                 there[u] = r < kt && pg < a.kv.pages;
                 const uint64_t row = pg * a.kv.page_stride + ((base + r) & mask) * a.kv.slot_stride + hk * a.kv.head_stride;
                 x[u] = *reinterpret_cast<const u32x4*>(a.kv.v + (there[u] ? row + 8u * (lane % lanes) : 0u));
+                if (f32) y[u] = *reinterpret_cast<const u32x4*>(a.kv.k + (there[u] ? row + 8u * (lane % lanes) : 0u));
             }
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u) {
-                bool bad = false;
+                bool bad = false, infinite = false;
 #pragma unroll
                 for (uint32_t d = 0; d < 4; ++d)
-                    bad = bad || (x[u][d] & 0x7fffu) >= infinity || ((x[u][d] >> 16) & 0x7fffu) >= infinity;
+#pragma unroll
+                    for (uint32_t half = 0; half < 32u; half += 16u) {
+                        const uint32_t v = (x[u][d] >> half) & 0x7fffu;
+                        bad = bad || v >= infinity;
+                        infinite = infinite || v == infinity || (f32 && ((y[u][d] >> half) & 0x7fffu) == infinity);
+                    }
+                if (infinite && there[u]) odd.infinite = 1u;
                 const uint32_t i = base + r0 + u * rows;
                 if (bad && there[u]) {
                     odd.end = odd.end > i ? odd.end : i + 1u;
@@ -390,59 +403,69 @@ __device__ OddValues odd_values(const PagedAttentionArgs& a, const Piece& p, con
     }
     return odd;
 }
-// Of the rows f0 + i whose bit i of `nan` is set, those that do not see all odd positions.
+// Of the rows f0 + i whose bit i of `nan` is set, those that have to be done again.
 __device__ __forceinline__ uint32_t rows_again(const PagedAttentionArgs& a, const Piece& p, uint32_t f0, uint32_t nan,
                                                const OddValues& odd) {
     const uint32_t i = threadIdx.x & 31u;
     const int32_t pos = p.len - static_cast<int32_t>(p.fresh) + static_cast<int32_t>(a.group(f0 + i));
     const bool hidden = static_cast<int32_t>(odd.end) > pos + 1 ||
                         (a.window && odd.first + a.window <= static_cast<uint32_t>(pos));
-    return static_cast<uint32_t>(__ballot(((nan >> i) & 1u) && hidden));
+    return static_cast<uint32_t>(__ballot(((nan >> i) & 1u) && (hidden || odd.infinite)));
 }
 
-// One row over the key tiles t0 .. t1 - 1 by one wave, reading only what the row sees.
-__device__ void row_alone(const PagedAttentionArgs& a, const Piece& p, const KeyTiles& keys, uint32_t kt, uint32_t t0,
-                          uint32_t t1, uint32_t hk, uint32_t f, const RowTo& to) {
+// One row over the key tiles t0 .. t1 - 1 by one wave, reading only what the row sees, in FP32.
+__device__ __forceinline__ void row_alone(const PagedAttentionArgs& a, const Piece& p, const KeyTiles& keys,
+                                          uint32_t kt, uint32_t t0, uint32_t t1, uint32_t hk, uint32_t f,
+                                          const RowTo& to) {
+    constexpr uint32_t U = 8u;
     const uint32_t lane = threadIdx.x & 63u, HD = a.kv.head_dim, token = p.q0 + a.group(f);
     const int32_t pos = p.len - static_cast<int32_t>(p.fresh) + static_cast<int32_t>(a.group(f));
     const uint64_t at = token * a.q_stride + (hk * a.group.by + a.group.rest(f)) * HD;
     const float c = a.scale * 1.4426950408889634f;
-    const uint32_t mask = (1u << a.kv.page_shift) - 1u;
+    const uint32_t mask = (1u << a.kv.page_shift) - 1u, column = 4u * lane % HD;
     const uint32_t* table = a.table + static_cast<uint64_t>(p.r) * a.table_stride;
     float m = -INFINITY, l = 0.0f;
     float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t t = t0; t < t1; ++t) {
+    for (uint32_t t = t0; t < t1 && l == l; ++t) {  // a sum that is NaN stays so
         const uint32_t i = keys.base(t, kt) + lane;
         uint32_t page = kNoSlot;
         if (lane < kt && row_sees(pos, i, a.window, a.sinks) && (i >> a.kv.page_shift) < a.table_stride)
             page = table[i >> a.kv.page_shift];
         const bool seen = page < a.kv.pages;
         const uint64_t row = seen ? page * a.kv.page_stride + (i & mask) * a.kv.slot_stride + hk * a.kv.head_stride : 0u;
-        float s = -INFINITY;
-        if (seen) {
-            s = 0.0f;
-            for (uint32_t d = 0; d < HD; ++d) {
-                const float q = a.type == T_F32 ? static_cast<const float*>(a.q)[at + d]
-                                                : cache_value(a.type, static_cast<const uint16_t*>(a.q)[at + d]);
-                s = fmaf(q, cache_value(a.kv.type, a.kv.k[row + d]), s);
+        const uint64_t all = __ballot(seen);
+        if (!all) continue;
+        float s = 0.0f;
+        for (uint32_t d = 0; d < HD; d += 8u) {
+            const u32x4 k = *reinterpret_cast<const u32x4*>(a.kv.k + row + d);
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                const float q = a.type == T_F32 ? static_cast<const float*>(a.q)[at + d + e]
+                                                : cache_value(a.type, static_cast<const uint16_t*>(a.q)[at + d + e]);
+                s = fmaf(q, cache_value(a.kv.type, static_cast<uint16_t>(k[e / 2u] >> (16u * (e % 2u)))), s);
             }
-            s *= c;
         }
+        s = seen ? s * c : -INFINITY;
         float top = s;
         for (uint32_t d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-        if (!__any(seen)) continue;
         const float next = fmaxf(m, top), ref = next == -INFINITY ? 0.0f : next;
-        const float e = seen ? exp2f(s - ref) : 0.0f, keep = exp2f(m - ref);
+        const float e = exp2f(s - ref), keep = exp2f(m - ref);
         float es = e;
         for (uint32_t d = 32; d > 0; d >>= 1) es += __shfl_xor(es, d);
         l = l * keep + es;
         for (uint32_t k = 0; k < 4u; ++k) o[k] *= keep;
-        for (uint32_t j = 0; j < kt; ++j) {
-            const float x = __shfl(e, j);
-            const uint64_t vr = __shfl(row, j);
-            if (x == 0.0f) continue;
-            for (uint32_t k = 0; k < 4u; ++k)
-                if (4u * lane + k < HD) o[k] = fmaf(x, cache_value(a.kv.type, a.kv.v[vr + 4u * lane + k]), o[k]);
+        for (uint32_t j = 0; j < kt; j += U) {
+            u32x2 v[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) v[u] = *reinterpret_cast<const u32x2*>(a.kv.v + __shfl(row, j + u) + column);
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                const float x = __shfl(e, j + u);
+                if (!((all >> (j + u)) & 1u)) continue;
+#pragma unroll
+                for (uint32_t k = 0; k < 4u; ++k)
+                    o[k] = fmaf(x, cache_value(a.kv.type, static_cast<uint16_t>(v[u][k / 2u] >> (16u * (k % 2u)))), o[k]);
+            }
         }
         m = next;
     }
@@ -531,7 +554,7 @@ struct RowsLds {
     alignas(16) uint64_t off[4][32];
     alignas(16) float o[4][16][HD + 4u];
     float m[4][16], l[4][16];
-    uint32_t nan, first, end;
+    uint32_t nan, first, end, infinite;
 };
 
 template <uint32_t T, uint32_t HD, bool F32>
@@ -548,7 +571,7 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
     if (!live_piece) return;
     if (tid == 0u) {
         write_head(a, w, p, hk);
-        lds.nan = lds.end = 0u;
+        lds.nan = lds.end = lds.infinite = 0u;
         lds.first = kNoPosition;
     }
     const uint32_t rows = p.fresh * a.group.by - p.tile * BM < BM ? p.fresh * a.group.by - p.tile * BM : BM;
@@ -702,7 +725,7 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
         lds.l[wave][j] = l;
     }
     __syncthreads();  // lds.nan is 0 as well
-    if (j < rows && l == l && any_nan(o)) atomicOr(&lds.nan, 1u << j);
+    if (j < rows && (l == l ? any_nan(o) : F32)) atomicOr(&lds.nan, 1u << j);
     {
         const float mm = fmaxf(fmaxf(lds.m[0][j], lds.m[1][j]), fmaxf(lds.m[2][j], lds.m[3][j]));
         const float keep = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mm);
@@ -724,8 +747,9 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
         const OddValues odd = odd_values(a, p, keys, KT, b0 + wave, b1, 4u, hk, lo, p_last);
         atomicMax(&lds.end, odd.end);
         atomicMin(&lds.first, odd.first);
+        atomicOr(&lds.infinite, odd.infinite);
         __syncthreads();
-        again = rows_again(a, p, p.tile * BM, again, {lds.first, lds.end});
+        again = rows_again(a, p, p.tile * BM, again, {lds.first, lds.end, lds.infinite});
     }
     if (row < rows && !((again >> row) & 1u)) {
         const RowTo to = row_to(a, w, p, BM, hk, row);
@@ -781,7 +805,7 @@ __device__ __forceinline__ void load_to_lds(const void* src, uint32_t offset, ui
 template <uint32_t HD>
 struct TilesLds {
     alignas(1024) uint8_t k[2][kTileKeys * 2u * HD], v[2][kTileKeys * 2u * HD];
-    uint32_t nan, first, end;
+    uint32_t nan, first, end, infinite;
 };
 
 template <uint32_t T, uint32_t HD, bool F32>
@@ -799,7 +823,7 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
     if (!live_piece) return;
     if (tid == 0u) {
         write_head(a, w, p, hk);
-        lds.nan = lds.end = 0u;
+        lds.nan = lds.end = lds.infinite = 0u;
         lds.first = kNoPosition;
     }
     const uint32_t left = p.fresh * a.group.by - p.tile * BM, rows = left < BM ? left : BM;
@@ -975,7 +999,7 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
             }
     }
     l += __shfl_xor(l, 32u);
-    const uint64_t either = __ballot(live && l == l && any_nan(o));
+    const uint64_t either = __ballot(live && (l == l ? any_nan(o) : F32));
     const uint32_t nan = static_cast<uint32_t>(either | (either >> 32));
     if (nan && lane == 0u) atomicOr(&lds.nan, 1u);  // (a barrier of the loop ago it was set to 0)
     if (live) {
@@ -991,9 +1015,10 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
     const OddValues odd = odd_values(a, p, keys, KT, t0 + wave, t1, 4u, hk, lo, p_last);
     atomicMax(&lds.end, odd.end);
     atomicMin(&lds.first, odd.first);
+    atomicOr(&lds.infinite, odd.infinite);
     __syncthreads();
     // (the stores of the rows that are done again came before the barrier)
-    uint32_t again = rows_again(a, p, f0, nan, {lds.first, lds.end});
+    uint32_t again = rows_again(a, p, f0, nan, {lds.first, lds.end, lds.infinite});
     while (again) {
         const uint32_t i = static_cast<uint32_t>(__builtin_ctz(again));
         again &= again - 1u;

@@ -1,5 +1,5 @@
 """Infinities and NaN in the paged attention, against plain 64-bit numpy: what masked positions
-hold does not matter."""
+hold does not matter, what visible ones hold counts as the definition says."""
 import numpy as np
 import pytest
 
@@ -74,6 +74,93 @@ def test_a_seen_nan_does_not_hide_a_masked_one(hip, gtype, cache, new, bad):
     close(c, got, rows, columns=rest)
     assert torch.isnan(got[:new, :2, 5]).all()
     assert torch.isfinite(got[rows, 2:, 5].float()).all()
+
+
+# ---- visible infinities ---------------------------------------------------------------
+
+def visible(c, hidden, window=0):
+    """attention_case's call in 64 bits, without the positions `hidden` of every request and
+    with V's infinities as 0."""
+    q, k, v = f64(c["q"]), f64(c["k"].nan_to_num(0, 0, 0)), f64(c["v"].nan_to_num(0, 0, 0))
+    out, tol = np.zeros_like(q), np.zeros_like(q)
+    for r, n in enumerate(c["lens"]):
+        for j in range(c["new"][r]):
+            t, p = int(c["start"][r]) + j, n - c["new"][r] + j
+            i = np.array([x for x in range(max(0, p + 1 - window) if window else 0, p + 1) if x not in hidden])
+            at = c["table"][r, i // c["page"]].astype(np.int64), i % c["page"]
+            for h in range(c["heads"]):
+                kk, vv = (x[at[0], at[1], h * c["kvh"] // c["heads"]] for x in (k, v))
+                s = kk @ q[t, h] * c["dim"] ** -0.5
+                w = np.exp(s - s.max())
+                out[t, h] = w @ vv / w.sum()
+                bound = np.array([np.abs(kk * q[t, h]).sum(-1).max() * c["dim"] ** -0.5, np.abs(vv).max(), len(i)])
+                tol[t, h] = P.attention_tolerance(out[t, h], bound, c["dim"], c["gtype"], c["cache"])
+    return out, tol
+
+
+@pytest.mark.parametrize("gtype,cache", TYPES)
+@pytest.mark.parametrize("dim", (64, 128, 256))
+@pytest.mark.parametrize("new", ([1, 1], [3, 1], [70, 40]))
+def test_visible_infinities(hip, gtype, cache, dim, new):
+    """A key of -inf where q is positive has no weight; a value of +-inf makes its column so."""
+    c = attention_case(73, [200, 90], new, 4, 2, dim, gtype, cache, 16)
+    c["q"][..., 7] = c["q"][..., 7].abs() + 0.25
+    for r in range(2):
+        for i in (5, 15):
+            c["k"][slot(c, r, i)][:, 7] = -INF
+        c["v"][slot(c, r, 9)][:, 3] = INF
+        c["v"][slot(c, r, 12)][:, 11] = -INF
+    want, tol = visible(c, {5, 15})
+    got = run_attention(hip, c)[:sum(new)].float()
+    assert (got[..., 3] == INF).all() and (got[..., 11] == -INF).all()
+    rest = [i for i in range(dim) if i not in (3, 11)]
+    off = np.abs(got.cpu().numpy().astype(np.float64) - want[:sum(new)])[..., rest]
+    assert np.all(np.isfinite(off)) and np.all(off <= tol[:sum(new)][..., rest])
+
+
+@pytest.mark.parametrize("gtype,cache", TYPES)
+@pytest.mark.parametrize("new", ([1], [40]))
+def test_visible_infinities_in_long_contexts(hip, gtype, cache, new):
+    """The same in one of a long row's parts, and in whole tiles and cut ones."""
+    c = attention_case(74, [5000], new, 2, 1, 64, gtype, cache, 16)
+    c["q"][..., 7] = c["q"][..., 7].abs() + 0.25
+    keys = {100, 2047, 4950}
+    for i in keys:
+        c["k"][slot(c, 0, i)][:, 7] = -INF
+    c["v"][slot(c, 0, 3001)][:, 3] = INF
+    want, tol = visible(c, keys)
+    got = run_attention(hip, c)[:sum(new)].float()
+    assert (got[..., 3] == INF).all()
+    rest = [i for i in range(64) if i != 3]
+    off = np.abs(got.cpu().numpy().astype(np.float64) - want[:sum(new)])[..., rest]
+    assert np.all(np.isfinite(off)) and np.all(off <= tol[:sum(new)][..., rest])
+
+
+@pytest.mark.parametrize("gtype", ("F16", "F32"))
+@pytest.mark.parametrize("new", ([1], [40]))
+def test_infinity_of_a_small_weight(hip, gtype, new):
+    """A weight that F16 cannot hold beside the row's largest still makes infinity of it."""
+    c = attention_case(75, [90], new, 2, 1, 64, gtype, "F16", 16)
+    c["q"][..., 7] = 8.0
+    c["k"][slot(c, 0, 20)][:, 7] = -40.0  # 40 below the others: a weight of about 2^-57
+    c["v"][slot(c, 0, 20)][:, 3] = INF
+    got = run_attention(hip, c)[:sum(new)].float()
+    assert (got[..., 3] == INF).all() and torch.isfinite(got[..., 4:]).all()
+
+
+@pytest.mark.parametrize("gtype,cache", TYPES)
+def test_no_score_above_minus_infinity(hip, gtype, cache):
+    """A row all of whose scores are -inf is 0, its neighbours that see more are not."""
+    c = attention_case(79, [3, 5], [3, 1], 4, 2, 64, gtype, cache, 16)
+    c["q"][..., 7] = c["q"][..., 7].abs() + 0.25
+    for r, i in ((0, 0), (0, 1), (1, 0), (1, 1), (1, 2), (1, 3), (1, 4)):
+        c["k"][slot(c, r, i)][:, 7] = -INF
+    got = run_attention(hip, c)
+    assert (got[[0, 1, 3]] == 0).all()
+    v = c["v"][slot(c, 0, 2)].float().repeat_interleave(2, 0)
+    # w v / w of one weight w: F32's parts hold 22 bits of it (four half steps of FP32), the sum
+    # of their products, 1 / w and its product lose a half step each; 16-bit types end on v
+    assert torch.all((got[2].float() - v).abs() <= 8 * 2.0 ** -24 * v.abs())
 
 
 # ---- what a NaN that rows see costs ---------------------------------------------------
