@@ -55,9 +55,18 @@ template <> struct Mat<T_BF16> {
 
 constexpr uint32_t parts_of(uint32_t T, bool f32) { return !f32 ? 1u : T == T_F16 ? 2u : 3u; }
 
-// The maximum moves (and o and l are rescaled) only when it has grown by 2^3; weights are
-// at most 2^(kBias + 3), inside F16.
-constexpr float kBias = 12.0f, kSlack = 3.0f;
+// The maximum moves (and o and l are rescaled) only when it has grown by 2^3, and weights carry
+// 2^bias: at most 2^(bias + 3).  F16: 2^15, so that small ones keep their bits, and with V at
+// most 2^16 FP32 holds any sum.  BF16, whose V may be as large as FP32's values: over the
+// len positions of a request, len 2^(bias + 3) is at most 1, so that no sum is above V's
+// largest, as with a softmax's weights.
+constexpr float kSlack = 3.0f;
+template <uint32_t T>
+__device__ __forceinline__ float weight_bias(int32_t len) {
+    if (T == T_F16) return 12.0f;
+    const float b = static_cast<float>(__builtin_clz(static_cast<uint32_t>(len) | 1u)) - 32.0f - kSlack;
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(b)));  // the same for all lanes
+}
 
 // 8 values as NP parts: v = parts[0] + parts[1] + ...
 template <typename M, uint32_t NP>
@@ -415,7 +424,7 @@ __device__ __forceinline__ uint32_t rows_again(const PagedAttentionArgs& a, cons
 
 // One row over the key tiles t0 .. t1 - 1 by one wave, reading only what the row sees, in FP32.
 __device__ __forceinline__ void row_alone(const PagedAttentionArgs& a, const Piece& p, const KeyTiles& keys,
-                                          uint32_t kt, uint32_t t0, uint32_t t1, uint32_t hk, uint32_t f,
+                                          uint32_t kt, uint32_t t0, uint32_t t1, uint32_t hk, uint32_t f, float bias,
                                           const RowTo& to) {
     constexpr uint32_t U = 8u;
     const uint32_t lane = threadIdx.x & 63u, HD = a.kv.head_dim, token = p.q0 + a.group(f);
@@ -449,7 +458,7 @@ __device__ __forceinline__ void row_alone(const PagedAttentionArgs& a, const Pie
         float top = s;
         for (uint32_t d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
         const float next = fmaxf(m, top), ref = next == -INFINITY ? 0.0f : next;
-        const float e = exp2f(s - ref), keep = exp2f(m - ref);
+        const float e = exp2f(s - ref + bias), keep = exp2f(m - ref);
         float es = e;
         for (uint32_t d = 32; d > 0; d >>= 1) es += __shfl_xor(es, d);
         l = l * keep + es;
@@ -469,8 +478,7 @@ __device__ __forceinline__ void row_alone(const PagedAttentionArgs& a, const Pie
         }
         m = next;
     }
-    // the other rows' sums are 2^kBias times as large under the same m
-    if (4u * lane < HD) store_row4(a, to, 4u * lane, f32x4{o[0], o[1], o[2], o[3]}, m + kBias, l);
+    if (4u * lane < HD) store_row4(a, to, 4u * lane, f32x4{o[0], o[1], o[2], o[3]}, m, l);
 }
 
 __device__ __forceinline__ float max_over(float v, uint32_t d) { return fmaxf(v, __shfl_xor(v, d)); }
@@ -588,6 +596,7 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
     const int32_t pos = live ? p0 + static_cast<int32_t>(a.group(f)) : -1;
     V8 q[NP][KK];
     float c = a.scale * 1.4426950408889634f;
+    const float bias = weight_bias<T>(p.len);
     load_q<T, F32, KK, 32u, 16u>(a, (p.q0 + (live ? a.group(f) : 0u)) * a.q_stride +
                                     (hk * a.group.by + (live ? a.group.rest(f) : 0u)) * HD + 8u * g, live, q, c);
     const uint32_t* table = a.table + static_cast<uint64_t>(p.r) * a.table_stride;
@@ -695,7 +704,7 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
 #pragma unroll
             for (uint32_t e = 0; e < DPL; ++e) o[e] = o[e] * keep;
         }
-        const float ref = m == -INFINITY ? 0.0f : m - kBias;
+        const float ref = m == -INFINITY ? 0.0f : m - bias;
         float pw[8];
 #pragma unroll
         for (uint32_t x = 0; x < 8; ++x) {
@@ -764,7 +773,7 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
     }
     if (again)
         for (uint32_t i = wave; i < rows; i += 4u)
-            if ((again >> i) & 1u) row_alone(a, p, keys, KT, b0, b1, hk, p.tile * BM + i, row_to(a, w, p, BM, hk, i));
+            if ((again >> i) & 1u) row_alone(a, p, keys, KT, b0, b1, hk, p.tile * BM + i, bias, row_to(a, w, p, BM, hk, i));
 }
 
 // ---------------------------------------------------------------------------
@@ -845,6 +854,7 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
     const int32_t pos = live ? p0 + static_cast<int32_t>(a.group(f)) : -1;
     V8 q[NP][KK];
     float c = a.scale * 1.4426950408889634f;
+    const float bias = weight_bias<T>(p.len);
     load_q<T, F32, KK, 16u, 32u>(a, (p.q0 + (live ? a.group(f) : 0u)) * a.q_stride +
                                     (hk * a.group.by + (live ? a.group.rest(f) : 0u)) * HD + 8u * h, live, q, c);
     // Loads: the wave brings 16 rows, a lane 16 bytes of a row at a time.  Lane i asks the table
@@ -974,7 +984,7 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
 #pragma unroll
             for (uint32_t d = 0; d < DT; ++d) o[d] = o[d] * keep;
         }
-        const float ref = m == -INFINITY ? 0.0f : m - kBias;
+        const float ref = m == -INFINITY ? 0.0f : m - bias;
 #pragma unroll
         for (uint32_t ks = 0; ks < 2; ++ks)
 #pragma unroll
@@ -1022,7 +1032,7 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
     while (again) {
         const uint32_t i = static_cast<uint32_t>(__builtin_ctz(again));
         again &= again - 1u;
-        row_alone(a, p, keys, KT, t0, t1, hk, f0 + i, row_to(a, w, p, BM, hk, 32u * wave + i));
+        row_alone(a, p, keys, KT, t0, t1, hk, f0 + i, bias, row_to(a, w, p, BM, hk, 32u * wave + i));
     }
 }
 

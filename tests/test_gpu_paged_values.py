@@ -1,10 +1,11 @@
-"""Infinities and NaN in the paged attention, against plain 64-bit numpy: what masked positions
-hold does not matter, what visible ones hold counts as the definition says."""
+"""Infinities, NaN and the ends of the types' ranges in the paged attention, against plain 64-bit
+numpy: what masked positions hold does not matter, what visible ones hold counts as the
+definition says."""
 import numpy as np
 import pytest
 
 from tests import paged as P
-from tests.test_gpu_paged import TYPES, attention_call, attention_case, f64, run_attention
+from tests.test_gpu_paged import TYPES, attention_call, attention_case, check_attention, f64, run_attention
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -161,6 +162,28 @@ def test_no_score_above_minus_infinity(hip, gtype, cache):
     # w v / w of one weight w: F32's parts hold 22 bits of it (four half steps of FP32), the sum
     # of their products, 1 / w and its product lose a half step each; 16-bit types end on v
     assert torch.all((got[2].float() - v).abs() <= 8 * 2.0 ** -24 * v.abs())
+
+
+# ---- the ends of the range ------------------------------------------------------------
+
+@pytest.mark.parametrize("gtype", ("BF16", "F32"))
+@pytest.mark.parametrize("dim", (64, 128))
+@pytest.mark.parametrize("lens,new", [([300, 4000], [1, 1]), ([300, 4000], [70, 40])])
+def test_largest_values(hip, gtype, dim, lens, new):
+    """Values near the end of BF16's range: their mean is in it."""
+    c = attention_case(76, lens, new, 4, 2, dim, gtype, "BF16", 16)
+    v = c["v"]
+    v[torch.isfinite(v)] = (2.0 ** 127 * (1.25 + 0.25 * torch.tanh(v[torch.isfinite(v)].float()))).bfloat16()
+    check_attention(c, run_attention(hip, c))
+
+
+@pytest.mark.parametrize("gtype", ("BF16", "F32"))
+@pytest.mark.parametrize("new", ([1, 1], [70, 40]))
+def test_small_values(hip, gtype, new):
+    """Small values keep their bits: the same call with values 2^-70 times as large."""
+    c = attention_case(77, [300, 4000], new, 4, 2, 64, gtype, "BF16", 16)
+    small = {**c, "v": (c["v"].float() * 2.0 ** -70).bfloat16()}
+    assert torch.equal(run_attention(hip, c)[:sum(new)], run_attention(hip, small)[:sum(new)] * 2.0 ** 70)
 
 
 # ---- what a NaN that rows see costs ---------------------------------------------------
