@@ -29,11 +29,13 @@ EXPF_TABLE = os.path.join(HERE, "libm_expf.bin")
 # kernel arrive in SGPRs with the wave instead of through a load of the
 # argument block (the code object keeps the loading path for firmware that
 # does not preload).
+# What the compiler says about inline assembly (a register it does not keep, for
+# instance) ends the build.
 HIP_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++20", "-fPIC", "-ffp-contract=off",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-mllvm", "-amdgpu-kernarg-preload-count=16",
-    "-Wall", "-Wno-unused-function", "-Wno-unknown-pragmas",
+    "-Wall", "-Wno-unused-function", "-Wno-unknown-pragmas", "-Werror=inline-asm",
 ]
 
 

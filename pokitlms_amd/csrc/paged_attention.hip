@@ -801,14 +801,14 @@ typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
 typedef uint8_t __attribute__((address_space(3))) * lds_ptr;
 
 // 16 bytes per lane from src (+ a lane's offset) into LDS, lane after lane from `to` (the
-// same for all lanes).  Written out, since the builtin makes every later LDS read wait for it:
-// the loop waits itself, once per tile, before the barrier that lets the tile be read.
+// same for all lanes), which the instruction takes in m0.  Written out, since the builtin
+// makes every later LDS read wait for it: the loop waits itself, once per tile, before the
+// barrier that lets the tile be read.
 __device__ __forceinline__ void load_to_lds(const void* src, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(to) : "memory", "m0");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(to) : "memory");
 }
 __device__ __forceinline__ void load_to_lds(const void* src, uint32_t offset, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(src), "s"(to)
-                 : "memory", "m0");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(src), "{m0}"(to) : "memory");
 }
 
 template <uint32_t HD>
