@@ -627,7 +627,8 @@ pk_hip_status pk_hip_paged_append_async(pk_hip_ctx* ctx, const pk_hip_paged_appe
  * rounded to the cache's type).  Requests with more than max_new rows, and rows of no
  * request, are left as they were.  What masked positions hold, NaN too, does not
  * matter; infinities that a row sees count as the formula says in FP32, and a row of
- * which every score is -inf as one that sees nothing. */
+ * which every score is -inf as one that sees nothing.  Calls of more tiles than a launch
+ * holds (2^24; 16 or 128 rows of one KV head's query heads each) return UNSUPPORTED. */
 typedef struct pk_hip_paged_attention {
     pk_hip_paged_kv cache;
     uint32_t type;               /* of q and out */

@@ -2449,6 +2449,8 @@ pk_hip_status pk_hip_paged_attention_async(pk_hip_ctx* ctx, const pk_hip_paged_a
     return guarded(ctx, err, cap, [&] {
         pk::PagedAttentionArgs a;
         require(pk::check_attention(attention, a));
+        if (pk::paged_attention_workgroups(a) > pk::kMaxPagedWorkgroups)
+            throw Unsupported("requests, tokens and KV heads make more tiles than a launch holds");
         require_usable(ctx);
         std::lock_guard lock(ctx->mutex);
         enqueue_paged(ctx, stream, ctx->stats.paged_attention_calls, ctx->stats.paged_attention_ns,

@@ -80,6 +80,9 @@ struct PagedAttentionArgs {
 // work: paged_attention_work_floats(a) floats of scratch, 16-byte aligned.
 size_t paged_attention_work_floats(const PagedAttentionArgs& a);
 uint32_t paged_attention_launches(const PagedAttentionArgs& a);
+// Of 256 threads, in the call's largest launch; a launch holds fewer than 2^32 threads.
+uint64_t paged_attention_workgroups(const PagedAttentionArgs& a);
+constexpr uint64_t kMaxPagedWorkgroups = (1ull << 24) - 1u;
 hipError_t launch_paged_attention(const PagedAttentionArgs& a, float* work, hipStream_t stream);
 
 // One step of a batched generation (prompt.hip): `rows` rows of plan.requests slots, whose

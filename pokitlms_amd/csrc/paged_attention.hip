@@ -1263,7 +1263,6 @@ void halves(const PagedAttentionArgs& a, Half& few, Half& many) {
 template <uint32_t T, uint32_t HD, bool F32>
 hipError_t attention_t(const PagedAttentionArgs& a, const Half& few, const Half& many, hipStream_t s) {
     const uint64_t fu = few.used ? few.units(a.kv.kv_heads) : 0u, mu = many.used ? many.units(a.kv.kv_heads) : 0u;
-    if (fu + mu >= (1ull << 31)) return hipErrorInvalidValue;
     const dim3 g(static_cast<uint32_t>(fu + mu)), b(256);
     if (few.w.schedule || many.w.schedule)
         hipLaunchKernelGGL(k_paged_schedule, dim3(2), dim3(1024), 0, s, a, few.w, many.w);
@@ -1291,6 +1290,12 @@ hipError_t attention_hd(const PagedAttentionArgs& a, const Half& few, const Half
 }
 
 }  // namespace
+
+uint64_t paged_attention_workgroups(const PagedAttentionArgs& a) {
+    Half few, many;
+    halves(a, few, many);
+    return (few.used ? few.units(a.kv.kv_heads) : 0u) + (many.used ? many.units(a.kv.kv_heads) : 0u);
+}
 
 uint32_t paged_attention_launches(const PagedAttentionArgs& a) {
     Half few, many;
