@@ -197,6 +197,8 @@ class Qwen3MoeModel:
         counts = [int(n_new)] * len(ps) if np.ndim(n_new) == 0 else [int(n) for n in n_new]
         if len(counts) != len(ps):
             raise ValueError("n_new needs one number per prompt")
+        if not all(0 <= n < 1 << 32 for n in counts):
+            raise ValueError("n_new counts new tokens, from 0 on and below 2^32")
         outs = [np.zeros(max(n, 1), np.uint32) for n in counts]
         logits = [np.zeros(self.shape.vocab, np.float32) for _ in ps] if want_logits else None
         reqs = (_abi.BatchRequest * max(len(ps), 1))(*[

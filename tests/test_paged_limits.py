@@ -23,3 +23,11 @@ def test_more_tiles_than_a_launch_holds(kw, kv):
 def test_large_calls_that_a_launch_holds(kw, kv):
     got = call("pk_hip_paged_attention_async", attention(cache(**kv), **kw))
     assert got[0] == 1 and OK in got[1], got
+
+
+@pytest.mark.parametrize("n_new", (-1, (1 << 32) + 1, [2, -3]))
+def test_counts_of_a_batch_that_are_no_counts(n_new):
+    """Refused before they are cut to 32 bits (no model is needed for that)."""
+    from pokitlms_amd.model import Qwen3MoeModel
+    with pytest.raises(ValueError, match="n_new"):
+        object.__new__(Qwen3MoeModel).generate_batch([[1, 2], [3]], n_new)
