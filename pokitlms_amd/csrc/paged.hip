@@ -430,9 +430,16 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppendArgs a) {
     }
 }
 
+// From this many tokens on a workgroup takes four, which spreads its start over more rows; with
+// fewer, more workgroups wait at once.  One token a workgroup or four, us: 32 + 4 heads of 128,
+// F16, 1024 tokens 6.7 and 9.0, 2048 10.0 and 11.8, 4096 17.2 and 16.6, 8192 28.5 and 28.7;
+// 16 + 2 of 256, BF16, 2048 9.8 and 12.0, 4096 16.8 and 16.8; 8 + 2 of 128, F16, 2048 5.1 and
+// 5.7, 4096 8.5 and 7.6, 8192 14.8 and 11.5.
+constexpr uint32_t kAppendManyTokens = 4096;
+
 template <uint32_t T, uint32_t HD>
 hipError_t append_t(const PagedAppendArgs& a, hipStream_t s) {
-    if (a.tokens < 1024u) hipLaunchKernelGGL((k_paged_append<T, HD, 1>), dim3(a.tokens), dim3(256), 0, s, a);
+    if (a.tokens < kAppendManyTokens) hipLaunchKernelGGL((k_paged_append<T, HD, 1>), dim3(a.tokens), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((k_paged_append<T, HD, 4>), dim3((a.tokens + 3u) / 4u), dim3(256), 0, s, a);
     return hipGetLastError();
 }
