@@ -409,8 +409,10 @@ typedef struct pk_hip_batch_request {
  * gives its pages to the next.  Each request's tokens and logits are those of its own
  * pk_hip_qwen3moe_generate within FP32 reassociation (fast mode; the same window of
  * kv_capacity positions).  Reference-order models and those whose prompts are not batched
- * return UNSUPPORTED.  Memory for the pages is taken for the call; where it is short, fewer
- * requests are on their way at once.  stats: prefill_ns wall time until the last prompt
+ * return UNSUPPORTED.  Memory for the pages is taken for the call: a request holds
+ * those of all of its positions until it ends, also behind the window (the ring of
+ * pk_hip_qwen3moe_generate holds kv_capacity); where memory is short, fewer requests are on
+ * their way at once, and RUNTIME_ERROR says that not even one fits.  stats: prefill_ns wall time until the last prompt
  * is through, decode_ns wall time of the steps after it, sums of tokens and forwards. */
 pk_hip_status pk_hip_qwen3moe_generate_batch(pk_hip_qwen3moe* model, const pk_hip_batch_request* requests,
                                              uint32_t n_requests, pk_hip_generation_stats* stats,

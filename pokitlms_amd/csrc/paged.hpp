@@ -26,8 +26,8 @@ struct PagedKv {
     uint64_t page_stride, slot_stride, head_stride;
 };
 
-// Plan: see pk_hip_paged_plan in pokit_hip.h.  work: 2 * requests + 1 words of scratch
-// where the plan takes two launches (plan_work_words).
+// Plan: see pk_hip_paged_plan in pokit_hip.h.  work: 2 * requests words of scratch
+// where the plan takes two launches (paged_plan_work_words).
 struct PagedPlanArgs {
     uint32_t requests, page_shift, pages, table_stride, max_tokens;
     const uint32_t *lens, *new_lens, *release, *free_count;

@@ -16,7 +16,10 @@
 // FP32 rows enter the 16-bit products as parts, q = q0 + q1 (+ q2) and likewise the weights:
 // two F16 parts hold 22 bits (q under a power of two per row, weights times 2^12, so that
 // small ones keep them), three BF16 parts 24.  16-bit rows round the weights once to
-// the cache's type, half a step of the output's own rounding.
+// the cache's type, half a step each at most, so the output is off by half a step of
+// sum_i w_i |v_i| at most and then rounds to the same type itself.  Over BF16 the mean error
+// is 0.0022 of the output's, 0.0017 with unrounded weights; a second part of the weights
+// would take half as many matrix instructions again.
 #include <hip/hip_fp16.h>
 #include <math.h>
 
@@ -231,7 +234,7 @@ __device__ __forceinline__ bool find_piece(const PagedAttentionArgs& a, const Ro
            (p.parts == 1u || split_fits(p.split, p.slot, a.kv.kv_heads, 1u << w.log_target));
 }
 
-// What find_piece needs where there are more requests than lanes: a workgroup per kind of
+// What find_piece needs where there are more than kWaveRequests requests: a workgroup per kind of
 // tile, its threads a 1024th of the requests each.
 __global__ __launch_bounds__(1024) void k_paged_schedule(PagedAttentionArgs a, RowWork few, RowWork many) {
     __shared__ double s_work[16];

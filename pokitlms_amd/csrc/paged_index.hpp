@@ -35,7 +35,7 @@ inline Divide divide_by(uint32_t d) {
     return {d, static_cast<uint32_t>((1ull << (31u + s)) / d + 1u), 31u + s};
 }
 
-// Rows of request r's new tokens for one kv head, 0 for a request that is left out.
+// A request's new tokens (group rows each for one kv head), 0 for one that is left out.
 PK_BOTH uint32_t paged_new(uint32_t q0, uint32_t q1, uint32_t max_new, uint32_t max_tokens) {
     return q1 > q0 && q1 <= max_tokens && q1 - q0 <= max_new ? q1 - q0 : 0u;
 }
