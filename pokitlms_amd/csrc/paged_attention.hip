@@ -360,8 +360,8 @@ __device__ __forceinline__ bool any_nan(const V (&o)[N]) {
 // see, times the parts, is NaN where the score is -inf or the output infinite.  (So can a
 // weight that its type rounds to 0.)  Rows whose sums are NaN in the end are rare; then one
 // more look at V, for F32 rows at K too, finds the positions that hold NaN or infinities, and
-// the rows that do not see all of them, or all if there is an infinity, are done again by
-// themselves.  Sums that are NaN because of a NaN that a row sees are right, and cost that look.
+// the rows that do not see all of them, those whose own q has an infinite part, or all if
+// there is an infinity, are done again by themselves.  Sums that are NaN because of a NaN that a row sees are right, and cost that look.
 constexpr uint32_t kNoPosition = 0x7fffffffu;
 struct OddValues {
     uint32_t first, end;  // V's first position that a window can hide (or kNoPosition), its last one's + 1 (or 0)
@@ -416,13 +416,20 @@ __device__ __forceinline__ OddValues odd_values(const PagedAttentionArgs& a, con
     return odd;
 }
 // Of the rows f0 + i whose bit i of `nan` is set, those that have to be done again.
-__device__ __forceinline__ uint32_t rows_again(const PagedAttentionArgs& a, const Piece& p, uint32_t f0, uint32_t nan,
-                                               const OddValues& odd) {
-    const uint32_t i = threadIdx.x & 31u;
-    const int32_t pos = p.len - static_cast<int32_t>(p.fresh) + static_cast<int32_t>(a.group(f0 + i));
-    const bool hidden = static_cast<int32_t>(odd.end) > pos + 1 ||
-                        (a.window && odd.first + a.window <= static_cast<uint32_t>(pos));
-    return static_cast<uint32_t>(__ballot(((nan >> i) & 1u) && (hidden || odd.infinite)));
+__device__ __forceinline__ uint32_t rows_again(const PagedAttentionArgs& a, const Piece& p, uint32_t hk, uint32_t f0,
+                                               uint32_t nan, const OddValues& odd) {
+    const uint32_t i = threadIdx.x & 31u, token = a.group(f0 + i), HD = a.kv.head_dim;
+    const int32_t pos = p.len - static_cast<int32_t>(p.fresh) + static_cast<int32_t>(token);
+    const bool mine = (nan >> i) & 1u;
+    bool again = odd.infinite || static_cast<int32_t>(odd.end) > pos + 1 ||
+                 (a.window && odd.first + a.window <= static_cast<uint32_t>(pos));
+    if (a.type == T_F32 && mine && !again) {
+        const float* q = static_cast<const float*>(a.q) + (p.q0 + token) * a.q_stride +
+                         (hk * a.group.by + a.group.rest(f0 + i)) * HD;
+        // (values from here on are infinite as BF16; F16's parts come under a power of two)
+        for (uint32_t d = 0; d < HD; ++d) again = again || fabsf(q[d]) >= 0x1.ffp127f;
+    }
+    return static_cast<uint32_t>(__ballot(mine && again));
 }
 
 // One row over the key tiles t0 .. t1 - 1 by one wave, reading only what the row sees, in FP32.
@@ -761,7 +768,7 @@ __device__ __forceinline__ void rows_piece(const PagedAttentionArgs& a, const Ro
         atomicMin(&lds.first, odd.first);
         atomicOr(&lds.infinite, odd.infinite);
         __syncthreads();
-        again = rows_again(a, p, p.tile * BM, again, {lds.first, lds.end, lds.infinite});
+        again = rows_again(a, p, hk, p.tile * BM, again, {lds.first, lds.end, lds.infinite});
     }
     if (row < rows && !((again >> row) & 1u)) {
         const RowTo to = row_to(a, w, p, BM, hk, row);
@@ -1031,7 +1038,7 @@ __device__ __forceinline__ void tiles_piece(const PagedAttentionArgs& a, const R
     atomicOr(&lds.infinite, odd.infinite);
     __syncthreads();
     // (the stores of the rows that are done again came before the barrier)
-    uint32_t again = rows_again(a, p, f0, nan, {lds.first, lds.end, lds.infinite});
+    uint32_t again = rows_again(a, p, hk, f0, nan, {lds.first, lds.end, lds.infinite});
     while (again) {
         const uint32_t i = static_cast<uint32_t>(__builtin_ctz(again));
         again &= again - 1u;

@@ -164,6 +164,29 @@ def test_no_score_above_minus_infinity(hip, gtype, cache):
     assert torch.all((got[2].float() - v).abs() <= 8 * 2.0 ** -24 * v.abs())
 
 
+@pytest.mark.parametrize("gtype,cache", TYPES)
+@pytest.mark.parametrize("new", ([1, 1], [40, 3]))
+def test_infinite_queries(hip, gtype, cache, new):
+    """An infinity in q that makes -inf of every score gives 0, one that makes +inf of any NaN."""
+    c = attention_case(80, [90, 50], new, 4, 2, 64, gtype, cache, 16)
+    c["k"][..., 7] = -c["k"][..., 7].abs() - 0.5
+    c["k"][..., 9] = -c["k"][..., 9].abs() - 0.5
+    c["k"][slot(c, 1, 5)][:, 9] = 1.0
+    c["q"][:new[0], 1, 7] = INF
+    c["q"][new[0]:, 2, 9] = INF
+    got = run_attention(hip, c)
+    assert (got[:new[0], 1] == 0).all() and torch.isnan(got[new[0]:sum(new), 2]).all()
+    assert torch.isfinite(got[:new[0], [0, 2, 3]].float()).all()
+
+
+def test_largest_query(hip):
+    """The largest FP32 value, which as BF16 would be infinite, times the smallest K."""
+    c = attention_case(81, [70, 40], [1, 40], 2, 1, 64, "F32", "BF16", 16)
+    c["q"][..., 7] = torch.finfo(torch.float32).max
+    c["k"][..., 7] = torch.where(c["k"][..., 7].float() > 0, 2.0 ** -126, 2.0 ** -127).bfloat16()
+    check_attention(c, run_attention(hip, c))
+
+
 # ---- the ends of the range ------------------------------------------------------------
 
 @pytest.mark.parametrize("gtype", ("BF16", "F32"))
