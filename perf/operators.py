@@ -292,7 +292,16 @@ def _prepare_attention(case, seed):
                   out=(0.01 * torch.randn(rows, case["heads"], dim, device="cuda", generator=g)).to(dtype))
 
 
+_stream = None
+
+
 def prepare(case, seed):
+    global _stream
+    if own:  # a program's torch work and the framework's calls share a stream of the program's:
+        # torch's default one has handle 0, which names the framework's own
+        if _stream is None:
+            _stream = torch.cuda.Stream()
+        torch.cuda.set_stream(_stream)
     return {"plan": _prepare_plan, "append": _prepare_append,
             "attention": _prepare_attention}[case["kind"]](case, seed)
 
